@@ -122,6 +122,58 @@ int qgemm_fp8_block_scaled_gemm(int out_dtype, int a_layout, int b_layout, const
                                 size_t N, size_t K, qgemm_stream_t stream);
 
 /*
+ * Quantisation to FP8 e4m3 with a power-of-two scale for each block of 128 elements: the operands of
+ * qgemm_fp8_block_e8m0_gemm. (The reference's fp8_mm takes block-scaled operands,
+ * src/mix_gemm/hip_mix_gemm_kernel.cpp:425-439, and has no kernel that makes them.)
+ *   in: FP32, BF16 or FP16 [rows, cols], ld_in >= cols, base aligned to its element.
+ *   Row form (q and scale, both or neither NULL): q[r*ld_q + c], blocks of 128 consecutive columns of a row, the form of a
+ *     matrix whose product sums over its columns. block_rows = 1: scale[(c/128)*rows + r]; block_rows = 128: one scale for
+ *     each square of 128 x 128, scale[(c/128)*ceil(rows/128) + r/128].
+ *   Column form (qt and scale_t): the transpose, qt[c*ld_qt + r], blocks of 128 consecutive rows of a column, for a
+ *     product that sums over the rows: scale_t[(r/128)*cols + c], or with block_rows = 128 scale_t[(r/128)*ceil(cols/128) +
+ *     c/128], the same squares' scales and codes as the row form's.
+ *   Both are made from one read when both are wanted.
+ *   Scale byte e stands for 2^(e - 127) (ue8m0): the least power of two, from 2^-127 up, that holds the block's largest
+ *   magnitude within +-448; 127 for a block of zeros. code = round_to_nearest_even(x / scale). A block that holds an
+ *   infinity or a NaN becomes NaN as a whole: scale byte 255, every code 0x7f. A last block may be shorter than 128.
+ * Every rows, cols up to 8388480; nothing is written beyond rows and cols. Work goes to `stream`; no scratch is used.
+ */
+int qgemm_quantize_block(int in_dtype, const void* in, size_t ld_in, size_t rows, size_t cols, int block_rows, void* q,
+                         size_t ld_q, void* scale, void* qt, size_t ld_qt, void* scale_t, qgemm_stream_t stream);
+
+/*
+ * The column form (as qgemm_quantize_block with block_rows = 1) of a matrix held in row form with a scale per row and
+ * block: its values, code * scale, quantised anew over blocks of 128 rows. A training step that keeps a layer's input as the
+ * 8-bit codes its forward product used (an activation checkpoint of one byte an element) makes the second operand of the
+ * weight gradient from them with this call. No value that codes and scales can express overflows or loses a bit on the way.
+ */
+int qgemm_requantize_block(const void* q, size_t ld_q, const void* scale, size_t rows, size_t cols, void* qt, size_t ld_qt,
+                           void* scale_t, qgemm_stream_t stream);
+
+/*
+ * out[r*ld_out + c] = round(code * scale) in FP32, BF16 or FP16 (beyond the type's range: an infinity) of a matrix in row
+ * form; block_rows as it was quantised. Restores an 8-bit activation checkpoint.
+ */
+int qgemm_dequantize_block(int out_dtype, const void* q, size_t ld_q, const void* scale, int block_rows, size_t rows,
+                           size_t cols, void* out, size_t ld_out, qgemm_stream_t stream);
+
+/*
+ * FP8 e4m3 GEMM with power-of-two block scales, which the tensor cores apply themselves (qgemm_fp8_block_scaled_gemm
+ * takes any fp32 scales and rescales in CUDA cores, at half the rate):
+ *   C[m,n] (+)= sum_kb 2^(ea + eb - 254) sum_{k in block kb} A[m,k] B[n,k]
+ *   with 128-wide K blocks, ea = a_scale[kb*M + m] (a_block_rows = 1) or a_scale[kb*ceil(M/128) + m/128] (128), and eb the
+ *   same of B and N; fp32 accumulation, one rounding to out_dtype (BF16, FP16 or FP32). The same entry serves a layer's
+ *   forward product and, on column forms, both backward products.
+ *   accumulate != 0: the product is added to C, FP32 only (a gradient over several micro-batches).
+ *   A [M,K], B [N,K]: 16-byte aligned bases and leading dimensions that are multiples of 16; C: any ldc >= N.
+ * Any M, N, K >= 0 (K = 0: zeros, or C unchanged when accumulating). No library scratch is used, so calls on several
+ * streams are independent; results are reproducible. The first GEMM call on a device must not be inside a stream capture.
+ */
+int qgemm_fp8_block_e8m0_gemm(int out_dtype, const void* A, size_t lda, const void* a_scale, int a_block_rows, const void* B,
+                              size_t ldb, const void* b_scale, int b_block_rows, int accumulate, void* C, size_t ldc,
+                              size_t M, size_t N, size_t K, qgemm_stream_t stream);
+
+/*
  * out[c*ld_out + r] = in[r*ld_in + c] for 1- or 2-byte elements. Replaces matrix_transpose<T>
  * (src/include/matrix_transpose.h:3-4; src/transpose/transpose.cu:60-77). Any rows, cols >= 0;
  * ld_in >= cols, ld_out >= rows (elements). in and out must not overlap.
@@ -195,7 +247,7 @@ int qgemm_device_status(int* out4);
 /*
  * The QGEMM_* environment variables (tuning overrides for experiments: QGEMM_TILE_N, QGEMM_SPLIT_K,
  * QGEMM_GROUP_M, QGEMM_CTA_PAIR, QGEMM_RELAYOUT_B, QGEMM_MAX_CTAS, QGEMM_DIRECT_STORE, QGEMM_FULL_A_TILE,
- * QGEMM_TAIL_SPLIT, QGEMM_BALANCE, QGEMM_PREFETCH, QGEMM_KCLUSTER, QGEMM_KGROUP, QGEMM_EARLY_GROUPS, QGEMM_ONE_TILE, QGEMM_EVEN_RUNS, QGEMM_HOST_BANDS, QGEMM_HOST_BANDS_N) are
+ * QGEMM_TAIL_SPLIT, QGEMM_BALANCE, QGEMM_PREFETCH, QGEMM_KCLUSTER, QGEMM_KGROUP, QGEMM_EARLY_GROUPS, QGEMM_ONE_TILE, QGEMM_EVEN_RUNS, QGEMM_E8M0_TILE_M, QGEMM_E8M0_SLICES, QGEMM_HOST_BANDS, QGEMM_HOST_BANDS_N) are
  * read once, when the library is
  * loaded; this reads them again. Not meant to run concurrently with GEMM calls of other threads.
  */

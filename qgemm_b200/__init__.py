@@ -31,6 +31,7 @@ C_ABI_SYMBOLS = (
     "qgemm_fp8_block_scaled_gemm", "qgemm_quantize", "qgemm_gemm_multi_dst", "qgemm_peer_export",
     "qgemm_peer_open", "qgemm_peer_close", "qgemm_gemm_host", "qgemm_plan_query", "qgemm_host_band_schedule",
     "qgemm_gemm_host_resident_a", "qgemm_plan_query_ex", "qgemm_peer_alloc", "qgemm_peer_free", "qgemm_reload_env", "qgemm_test_arm_skip_load",
+    "qgemm_quantize_block", "qgemm_requantize_block", "qgemm_dequantize_block", "qgemm_fp8_block_e8m0_gemm",
 )
 
 
@@ -75,6 +76,14 @@ def lib() -> C.CDLL:
         L.qgemm_fp8_block_scaled_gemm.restype = i
         L.qgemm_quantize.argtypes = [i, i, vp, sz, vp, sz, fp, fp, sz, sz, vp]
         L.qgemm_quantize.restype = i
+        L.qgemm_quantize_block.argtypes = [i, vp, sz, sz, sz, i, vp, sz, vp, vp, sz, vp, vp]
+        L.qgemm_quantize_block.restype = i
+        L.qgemm_requantize_block.argtypes = [vp, sz, vp, sz, sz, vp, sz, vp, vp]
+        L.qgemm_requantize_block.restype = i
+        L.qgemm_dequantize_block.argtypes = [i, vp, sz, vp, i, sz, sz, vp, sz, vp]
+        L.qgemm_dequantize_block.restype = i
+        L.qgemm_fp8_block_e8m0_gemm.argtypes = [i, vp, sz, vp, i, vp, sz, vp, i, i, vp, sz, sz, sz, sz, vp]
+        L.qgemm_fp8_block_e8m0_gemm.restype = i
         L.qgemm_gemm_multi_dst.argtypes = [i, i, i, vp, sz, vp, sz, fp, fp, C.POINTER(C.c_void_p), i, sz, sz, sz, sz, vp]
         L.qgemm_gemm_multi_dst.restype = i
         L.qgemm_gemm_host.argtypes = [i, i, i, vp, sz, vp, sz, C.POINTER(C.c_float), C.POINTER(C.c_float), vp, sz, sz,
@@ -305,6 +314,181 @@ def fp8_block_mm(a, b, a_scale, b_scale, c, reference_layout: bool = True) -> No
             max(b.stride(0), b.shape[1]), a_scale.data_ptr(), b_scale.data_ptr(), c.data_ptr(), max(c.stride(0), N),
             M, N, K, _stream_ptr(a))
     _check(rc, "qgemm_fp8_block_scaled_gemm")
+
+
+# ------------------------------------------------------------------------ power-of-two block scales
+BLOCK = 128  #: elements of the summed axis that share a scale
+
+
+def _blocks(n: int) -> int:
+    return -(-n // BLOCK)
+
+
+def _same_device(what, *tensors):
+    if any(t.device != tensors[0].device for t in tensors):
+        raise QgemmError(ERR_INVALID_ARG, f"{what}: the tensors are on different devices")
+
+
+def _codes_empty(rows: int, cols: int, device):
+    """[rows, cols] e4m3 codes whose rows start on 16-byte boundaries, as the product reads them."""
+    torch = _torch()
+    return torch.empty((rows, -(-cols // 16) * 16), dtype=torch.float8_e4m3fn, device=device)[:, :cols]
+
+
+def _scale_block_rows(what: str, scale, rows: int, cols: int) -> int:
+    """1 or 128: how many rows of a row-form [rows, cols] matrix share one of ``scale``'s entries, by its shape."""
+    torch = _torch()
+    if not scale.is_cuda or scale.dtype != torch.float8_e8m0fnu or not scale.is_contiguous():
+        raise QgemmError(ERR_INVALID_ARG, f"{what} must be a contiguous float8_e8m0fnu CUDA tensor")
+    for block_rows, n in ((1, rows), (BLOCK, _blocks(rows))):
+        if tuple(scale.shape) == (_blocks(cols), n):
+            return block_rows
+    raise QgemmError(ERR_INVALID_ARG, f"{what} of a [{rows}, {cols}] matrix is [{_blocks(cols)}, {rows}] or "
+                     f"[{_blocks(cols)}, {_blocks(rows)}], got {list(scale.shape)}")
+
+
+def _require_codes(name, t, rows=None, cols=None):
+    torch = _torch()
+    _require_cuda_2d(name, t)
+    if t.dtype != torch.float8_e4m3fn or (rows is not None and tuple(t.shape) != (rows, cols)):
+        raise QgemmError(ERR_INVALID_ARG, f"{name} must be float8_e4m3fn" + (f" [{rows}, {cols}]" if rows is not None else ""))
+
+
+def _ld(t) -> int:
+    """Leading dimension of a 2-D tensor with unit inner stride; one row has none of its own."""
+    if t.shape[0] <= 1:
+        return -(-max(t.stride(0), t.shape[1]) // 16) * 16
+    return t.stride(0)
+
+
+def _code_form(form_rows: int, form_cols: int, square: bool, out, what: str, device):
+    """(codes, scales) of one form, allocated or checked."""
+    torch = _torch()
+    shape = (_blocks(form_cols), _blocks(form_rows) if square else form_rows)
+    if out is None:
+        return _codes_empty(form_rows, form_cols, device), torch.empty(shape, dtype=torch.float8_e8m0fnu, device=device)
+    q, s = out
+    _require_codes(f"{what} codes", q, form_rows, form_cols)
+    if not s.is_cuda or s.dtype != torch.float8_e8m0fnu or tuple(s.shape) != shape or not s.is_contiguous():
+        raise QgemmError(ERR_INVALID_ARG, f"{what} scales must be a contiguous float8_e8m0fnu CUDA tensor {list(shape)}")
+    if q.device != device or s.device != device:
+        raise QgemmError(ERR_INVALID_ARG, f"{what}: the tensors are on different devices")
+    if form_rows > 1 and q.stride(0) < form_cols:
+        raise QgemmError(ERR_INVALID_ARG, f"{what} codes: rows overlap")
+    return q, s
+
+
+def quantize_block(x, square: bool = False, form: str = "row", out=None):
+    """FP8 e4m3 codes of a bf16 / fp16 / fp32 CUDA matrix with a power-of-two scale for each block of 128 elements.
+
+    ``form="row"``: blocks lie along the rows, for a product that sums over x's columns. Returns ``(q, scale)``, ``q``
+    [rows, cols] float8_e4m3fn, ``scale`` [ceil(cols/128), rows] float8_e8m0fnu. ``form="column"``: blocks lie along the
+    columns, for a product that sums over x's rows: ``(qt, scale_t)`` of the transpose, [cols, rows] and
+    [ceil(rows/128), cols]. ``form="both"``: all four, from one read of x. With ``square`` one scale covers 128 x 128
+    (weights): ``scale`` [ceil(cols/128), ceil(rows/128)], and both forms hold the same codes.
+
+    The scale is the least power of two (2^-127 at least) with which the block's largest magnitude is at most 448; a
+    block holding an infinity or a NaN becomes NaN as a whole. New codes get rows that start on 16-byte boundaries (the
+    product asks for that); ``out`` takes the tensors of an earlier call to write into instead."""
+    torch = _torch()
+    _require_cuda_2d("x", x)
+    if form not in ("row", "column", "both"):
+        raise QgemmError(ERR_INVALID_ARG, f"form is 'row', 'column' or 'both', got {form!r}")
+    if x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise QgemmError(ERR_UNSUPPORTED, f"quantize_block of dtype {x.dtype}")
+    rows, cols = x.shape
+    if rows > 1 and x.stride(0) < cols:
+        raise QgemmError(ERR_INVALID_ARG, "quantize_block: the rows of x overlap")
+    n = 4 if form == "both" else 2
+    if out is not None and len(out) != n:
+        raise QgemmError(ERR_INVALID_ARG, f"out has {n} tensors with form={form!r}")
+    res = ()
+    q = s = qt = st = None
+    if form != "column":
+        q, s = _code_form(rows, cols, square, None if out is None else out[:2], "row form", x.device)
+        res += (q, s)
+    if form != "row":
+        qt, st = _code_form(cols, rows, square, None if out is None else out[-2:], "column form", x.device)
+        res += (qt, st)
+    with torch.cuda.device(x.device):
+        rc = lib().qgemm_quantize_block(
+            _dtype_code(x), x.data_ptr(), _ld(x), rows, cols, BLOCK if square else 1,
+            q.data_ptr() if q is not None else None, _ld(q) if q is not None else 0, s.data_ptr() if s is not None else None,
+            qt.data_ptr() if qt is not None else None, _ld(qt) if qt is not None else 0,
+            st.data_ptr() if st is not None else None, _stream_ptr(x))
+    _check(rc, "qgemm_quantize_block")
+    return res
+
+
+def requantize_block(q, scale, out=None):
+    """Column form ``(qt, scale_t)`` of a matrix held in row form with a scale per row and block: the values
+    code * scale quantised anew over blocks of 128 rows. Turns a saved 8-bit activation into the operand of the weight
+    gradient, dW = dy^T x. (A matrix with ``square`` scales needs no new codes: transpose codes and scales.)"""
+    torch = _torch()
+    _require_codes("q", q)
+    rows, cols = q.shape
+    if rows > 1 and q.stride(0) < cols:
+        raise QgemmError(ERR_INVALID_ARG, "requantize_block: the rows of q overlap")
+    if _scale_block_rows("scale", scale, rows, cols) != 1:
+        raise QgemmError(ERR_UNSUPPORTED, "requantize_block takes a scale per row; with square blocks transpose codes and scales")
+    _same_device("requantize_block", q, scale)
+    qt, st = _code_form(cols, rows, False, out, "column form", q.device)
+    with torch.cuda.device(q.device):
+        rc = lib().qgemm_requantize_block(q.data_ptr(), _ld(q), scale.data_ptr(), rows, cols, qt.data_ptr(), _ld(qt),
+                                          st.data_ptr(), _stream_ptr(q))
+    _check(rc, "qgemm_requantize_block")
+    return qt, st
+
+
+def dequantize_block(q, scale, out_dtype=None, out=None):
+    """code * scale of a row-form matrix, rounded to ``out_dtype`` (bf16 unless told otherwise; fp16, fp32)."""
+    torch = _torch()
+    _require_codes("q", q)
+    rows, cols = q.shape
+    if rows > 1 and q.stride(0) < cols:
+        raise QgemmError(ERR_INVALID_ARG, "dequantize_block: the rows of q overlap")
+    block_rows = _scale_block_rows("scale", scale, rows, cols)
+    if out is None:
+        out = torch.empty((rows, cols), dtype=out_dtype or torch.bfloat16, device=q.device)
+    _require_cuda_2d("out", out)
+    if tuple(out.shape) != (rows, cols) or (out_dtype is not None and out.dtype != out_dtype):
+        raise QgemmError(ERR_INVALID_ARG, "out must have q's shape and the requested dtype")
+    if out.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise QgemmError(ERR_UNSUPPORTED, f"dequantize_block to dtype {out.dtype}")
+    if rows > 1 and out.stride(0) < cols:
+        raise QgemmError(ERR_INVALID_ARG, "dequantize_block: the rows of out overlap")
+    _same_device("dequantize_block", q, scale, out)
+    with torch.cuda.device(q.device):
+        rc = lib().qgemm_dequantize_block(_dtype_code(out), q.data_ptr(), _ld(q), scale.data_ptr(), block_rows, rows, cols,
+                                          out.data_ptr(), _ld(out), _stream_ptr(q))
+    _check(rc, "qgemm_dequantize_block")
+    return out
+
+
+def fp8_block_mm_e8m0(a, b, a_scale, b_scale, c, accumulate: bool = False) -> None:
+    """c[m,n] = a[m,k] x b[n,k]^T of FP8 codes with power-of-two block scales (:func:`quantize_block`), the scales applied
+    by the tensor cores; argument order as :func:`fp8_block_mm`. ``a_scale`` [ceil(k/128), m] or, one for 128 rows,
+    [ceil(k/128), ceil(m/128)]; ``b_scale`` likewise of n. ``c`` bf16 / fp16 / fp32; ``accumulate`` adds to what a fp32 ``c``
+    holds. Rows of ``a`` and ``b`` start on 16-byte boundaries. A layer's three products, with x, w and dy quantised:
+    forward (x row, w row), dx = (dy row, w column), dw = (dy column, x column)."""
+    torch = _torch()
+    _require_codes("a", a)
+    _require_codes("b", b)
+    _require_cuda_2d("c", c)
+    M, K = a.shape
+    N = b.shape[0]
+    if b.shape[1] != K or tuple(c.shape) != (M, N):
+        raise QgemmError(ERR_INVALID_ARG, f"shape mismatch a{tuple(a.shape)} b{tuple(b.shape)} c{tuple(c.shape)}")
+    a_rows = _scale_block_rows("a_scale", a_scale, M, K)
+    b_rows = _scale_block_rows("b_scale", b_scale, N, K)
+    _same_device("fp8_block_mm_e8m0", a, b, a_scale, b_scale, c)
+    if M > 1 and c.stride(0) < N:
+        raise QgemmError(ERR_INVALID_ARG, "the rows of c overlap")
+    with torch.cuda.device(a.device):
+        rc = lib().qgemm_fp8_block_e8m0_gemm(
+            _dtype_code(c), a.data_ptr(), _ld(a), a_scale.data_ptr(), a_rows, b.data_ptr(), _ld(b), b_scale.data_ptr(), b_rows,
+            1 if accumulate else 0, c.data_ptr(), _ld(c), M, N, K, _stream_ptr(a))
+    _check(rc, "qgemm_fp8_block_e8m0_gemm")
 
 
 MAX_DSTS = 8  # QGEMM_MAX_DSTS

@@ -15,6 +15,7 @@
 #include <mutex>
 #include <unordered_map>
 
+#include "gemm_e8m0.cuh"
 #include "gemm_launch.cuh"
 #include "qgemm_internal.h"
 
@@ -234,6 +235,8 @@ EnvSettings read_env() {
     const char* ot = std::getenv("QGEMM_ONE_TILE");  // 0: never the one-tile-per-CTA kernel variants
     e.one_tile_off = (ot != nullptr && ot[0] == '0') ? 1 : 0;
     e.kgroup = std::max(0, env_int("QGEMM_KGROUP"));  // 0 = the library's choice, 1 = off, 2 / 4 / 8 = K blocks per load
+    e.e8m0_tile_m = std::max(0, env_int("QGEMM_E8M0_TILE_M"));  // tile rows of the power-of-two block-scaled GEMM
+    e.e8m0_slices = std::max(0, env_int("QGEMM_E8M0_SLICES"));  // its K slices
     e.host_bands = std::max(0, env_int("QGEMM_HOST_BANDS"));
     e.host_bands_n = std::max(0, env_int("QGEMM_HOST_BANDS_N"));
     return e;
@@ -930,6 +933,22 @@ int int4_dispatch(int out_dtype, int b_layout, const void* A, size_t lda, const 
                          K, tuning, stream);
 }
 
+// Tile and K slices of the power-of-two block-scaled GEMM.
+struct E8m0Plan {
+    int tile_m, tile_n, slices;
+};
+E8m0Plan plan_e8m0(size_t M, size_t N, int kb_total, int sms) {
+    E8m0Plan pl;
+    pl.tile_m = M <= 16 ? 16 : (M <= 32 ? 32 : (M <= 64 ? 64 : 128));
+    pl.tile_n = 128;
+    const long long tiles = static_cast<long long>((M + pl.tile_m - 1) / pl.tile_m) * static_cast<long long>((N + 127) / 128);
+    pl.slices = 1;
+    while (pl.slices < 8 && tiles * pl.slices * 2 <= 2ll * sms && kb_total >= pl.slices * 2) pl.slices *= 2;
+    if (g_env.e8m0_tile_m > 0) pl.tile_m = g_env.e8m0_tile_m;
+    if (g_env.e8m0_slices > 0) pl.slices = std::min(g_env.e8m0_slices, kb_total);
+    return pl;
+}
+
 int blockscale_dispatch(int out_dtype, int a_layout, int b_layout, const void* A, size_t lda, const void* B,
                         size_t ldb, const float* a_scale, const float* b_scale, void* C, size_t ldc, size_t M, size_t N,
                         size_t K, cudaStream_t stream) {
@@ -1012,6 +1031,65 @@ int blockscale_dispatch(int out_dtype, int a_layout, int b_layout, const void* A
     return launch_fp8_blockscale(out_kind, ta, tb, tc, p, grid, stream) == cudaSuccess ? QGEMM_OK : QGEMM_ERR_CUDA;
 }
 
+// FP8 GEMM with power-of-two block scales. No library scratch: calls on different streams are independent.
+int e8m0_dispatch(int out_dtype, const void* A, size_t lda, const uint8_t* a_scale, int a_block_rows, const void* B,
+                  size_t ldb, const uint8_t* b_scale, int b_block_rows, int accumulate, void* C, size_t ldc, size_t M,
+                  size_t N, size_t K, cudaStream_t stream) {
+    const int out_kind = out_kind_of(out_dtype);
+    if (out_kind != OUT_F32 && out_kind != OUT_BF16 && out_kind != OUT_F16) return QGEMM_ERR_UNSUPPORTED;
+    if (accumulate != 0 && out_kind != OUT_F32) return QGEMM_ERR_UNSUPPORTED;
+    if ((a_block_rows != 1 && a_block_rows != 128) || (b_block_rows != 1 && b_block_rows != 128)) return QGEMM_ERR_INVALID_ARG;
+    if (M == 0 || N == 0) return QGEMM_OK;
+    if (C == nullptr || ldc < N) return QGEMM_ERR_INVALID_ARG;
+    if (M > 0x7fffff00ull || N > 0x7fffff00ull || K > 0x7fffff00ull) return QGEMM_ERR_INVALID_ARG;
+    const size_t out_bytes = (out_kind == OUT_F32) ? 4 : 2;
+    if (reinterpret_cast<uintptr_t>(C) % out_bytes != 0) return QGEMM_ERR_ALIGNMENT;
+    if (K == 0) {  // an empty sum
+        if (accumulate != 0) return QGEMM_OK;
+        return cudaMemset2DAsync(C, ldc * out_bytes, 0, N * out_bytes, M, stream) == cudaSuccess ? QGEMM_OK : QGEMM_ERR_CUDA;
+    }
+    if (A == nullptr || B == nullptr || a_scale == nullptr || b_scale == nullptr || lda < K || ldb < K)
+        return QGEMM_ERR_INVALID_ARG;
+    if (reinterpret_cast<uintptr_t>(A) % 16 != 0 || lda % 16 != 0 || reinterpret_cast<uintptr_t>(B) % 16 != 0 || ldb % 16 != 0)
+        return QGEMM_ERR_ALIGNMENT;
+
+    std::lock_guard<std::mutex> lock(g_mutex);
+    DeviceState* st = nullptr;
+    int rc = get_state(&st);
+    if (rc != QGEMM_OK) return rc;
+
+    E8m0Params p;
+    std::memset(&p, 0, sizeof(p));
+    p.C = C;
+    p.ldc = static_cast<long long>(ldc);
+    p.M = static_cast<int>(M);
+    p.N = static_cast<int>(N);
+    p.K = static_cast<int>(K);
+    p.kb_total = static_cast<int>((K + 127) / 128);
+    p.a_scale = a_scale;
+    p.b_scale = b_scale;
+    p.a_shift = a_block_rows == 128 ? 7 : 0;
+    p.b_shift = b_block_rows == 128 ? 7 : 0;
+    p.a_rows = static_cast<long long>(a_block_rows == 128 ? (M + 127) / 128 : M);
+    p.b_rows = static_cast<long long>(b_block_rows == 128 ? (N + 127) / 128 : N);
+    p.out = out_kind;
+    p.accumulate = accumulate != 0;
+    p.status = st->status;
+    p.c_vec_ok = reinterpret_cast<uintptr_t>(C) % (4 * out_bytes) == 0 && ldc % 4 == 0;
+
+    const E8m0Plan plan = plan_e8m0(M, N, p.kb_total, st->sm_count);
+    CUtensorMap ta, tb;
+    p.m_tiles = static_cast<int>((M + plan.tile_m - 1) / plan.tile_m);
+    p.n_tiles = static_cast<int>((N + plan.tile_n - 1) / plan.tile_n);
+    if (static_cast<long long>(p.m_tiles) * p.n_tiles * 8 > 0x7fffffffLL) return QGEMM_ERR_UNSUPPORTED;
+    rc = make_operand_map(A, M, K, lda, QGEMM_DTYPE_FP8_E4M3, static_cast<uint32_t>(plan.tile_m), &ta);
+    if (rc != QGEMM_OK) return rc;
+    rc = make_operand_map(B, N, K, ldb, QGEMM_DTYPE_FP8_E4M3, 128u, &tb);
+    if (rc != QGEMM_OK) return rc;
+    p.idesc = ptx::make_idesc_e8m0(128u, static_cast<uint32_t>(plan.tile_m));
+    return launch_e8m0_small(plan.tile_m, plan.slices, ta, tb, p, stream) == cudaSuccess ? QGEMM_OK : QGEMM_ERR_CUDA;
+}
+
 }  // namespace
 
 std::mutex& dispatch_mutex() { return g_mutex; }
@@ -1073,6 +1151,32 @@ int qgemm_fp8_block_scaled_gemm(int out_dtype, int a_layout, int b_layout, const
                                 size_t N, size_t K, qgemm_stream_t stream) {
     return blockscale_dispatch(out_dtype, a_layout, b_layout, A, lda, B, ldb, a_scale, b_scale, C, ldc, M, N, K,
                                reinterpret_cast<cudaStream_t>(stream));
+}
+
+int qgemm_fp8_block_e8m0_gemm(int out_dtype, const void* A, size_t lda, const void* a_scale, int a_block_rows, const void* B,
+                              size_t ldb, const void* b_scale, int b_block_rows, int accumulate, void* C, size_t ldc,
+                              size_t M, size_t N, size_t K, qgemm_stream_t stream) {
+    return e8m0_dispatch(out_dtype, A, lda, static_cast<const uint8_t*>(a_scale), a_block_rows, B, ldb,
+                         static_cast<const uint8_t*>(b_scale), b_block_rows, accumulate, C, ldc, M, N, K,
+                         reinterpret_cast<cudaStream_t>(stream));
+}
+
+int qgemm_quantize_block(int in_dtype, const void* in, size_t ld_in, size_t rows, size_t cols, int block_rows, void* q,
+                         size_t ld_q, void* scale, void* qt, size_t ld_qt, void* scale_t, qgemm_stream_t stream) {
+    return quantize_block_launch(in_dtype, in, ld_in, rows, cols, block_rows, q, ld_q, static_cast<uint8_t*>(scale), qt, ld_qt,
+                                 static_cast<uint8_t*>(scale_t), reinterpret_cast<cudaStream_t>(stream));
+}
+
+int qgemm_requantize_block(const void* q, size_t ld_q, const void* scale, size_t rows, size_t cols, void* qt, size_t ld_qt,
+                           void* scale_t, qgemm_stream_t stream) {
+    return requantize_block_launch(q, ld_q, static_cast<const uint8_t*>(scale), rows, cols, qt, ld_qt,
+                                   static_cast<uint8_t*>(scale_t), reinterpret_cast<cudaStream_t>(stream));
+}
+
+int qgemm_dequantize_block(int out_dtype, const void* q, size_t ld_q, const void* scale, int block_rows, size_t rows,
+                           size_t cols, void* out, size_t ld_out, qgemm_stream_t stream) {
+    return dequantize_block_launch(out_dtype, q, ld_q, static_cast<const uint8_t*>(scale), block_rows, rows, cols, out, ld_out,
+                                   reinterpret_cast<cudaStream_t>(stream));
 }
 
 int qgemm_quantize(int in_dtype, int out_dtype, const void* in, size_t ld_in, void* out, size_t ld_out,

@@ -311,5 +311,71 @@ __device__ __forceinline__ void umma_ss_pair(uint32_t d_tmem, uint64_t a_desc, u
     }
 }
 
+// ---------------------------------------------------------------- block-scaled tcgen05.mma (kind::mxf8f6f4)
+// D (+)= sum_k (A[m,k] * SA[m]) * (B[n,k] * SB[n]) with ue8m0 scales in tensor memory: the instruction multiplies 32
+// bytes of K, one scale per row of either operand. A 32-bit word of tensor memory holds the scales of one row for four
+// such steps; the descriptor's two-bit scale ids (make_idesc_e8m0) choose the byte. Rows 32 j + lane of an operand lie in
+// column j of its scale region, repeated over the four lane quadrants.
+__device__ __forceinline__ void umma_e8m0(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                          uint32_t sa_tmem, uint32_t sb_tmem, uint32_t accumulate) {
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %6, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}\n"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sa_tmem), "r"(sb_tmem), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void umma_e8m0_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                               uint32_t sa_tmem, uint32_t sb_tmem, uint32_t accumulate) {
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %6, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}\n"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sa_tmem), "r"(sb_tmem), "r"(accumulate)
+        : "memory");
+}
+// Both operands e4m3 and K-major, scales ue8m0 (bit 23); bits [4,6) / [29,31): scale id of B / A.
+__host__ __device__ constexpr uint32_t make_idesc_e8m0(uint32_t m, uint32_t n) {
+    return ((n >> 3) << 17) | (1u << 23) | ((m >> 4) << 24);
+}
+__host__ __device__ constexpr uint32_t idesc_scale_id(uint32_t id) { return (id << 4) | (id << 29); }
+
+// Descriptor of 32 rows x 16 bytes laid end to end (no swizzle: groups of 8 rows 128 bytes apart), the source of
+// tc_copy_scales: row `lane` = the four words (rows lane, 32 + lane, 64 + lane, 96 + lane) of 128 rows' scales.
+__device__ __forceinline__ uint64_t make_scale_desc(uint32_t smem_addr) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
+    d |= static_cast<uint64_t>(128 >> 4) << 32;  // stride byte offset
+    d |= static_cast<uint64_t>(1) << 46;
+    return d;
+}
+// 512 bytes of shared memory to four columns of tensor memory, repeated over the four lane quadrants. Ordered before
+// the MMAs that the same thread issues after it; a tcgen05.commit covers it.
+__device__ __forceinline__ void tc_copy_scales(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// In both CTAs of the pair, each from its own shared memory.
+__device__ __forceinline__ void tc_copy_scales_pair(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// try_wait that also orders what another CTA of the cluster wrote before its arrival.
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+        "selp.u32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+// 3-D tiled fp32 add shared -> global: every element of the box is added once to the tensor's, clipped as a store is.
+__device__ __forceinline__ void tma_add_3d(const CUtensorMap* tmap, uint32_t src_smem, int x, int y, int z) {
+    asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3, %4}], [%1];"
+                 ::"l"(reinterpret_cast<uint64_t>(tmap)), "r"(src_smem), "r"(x), "r"(y), "r"(z)
+                 : "memory");
+}
+
 }  // namespace ptx
 }  // namespace qgemm

@@ -23,6 +23,15 @@ int splitk_reduce_launch(const void* partials, long long split_stride, long long
 int quantize_launch(int in_dtype, int out_dtype, const void* in, size_t ld_in, void* out, size_t ld_out,
                     float* scale_out, float* amax_out, size_t rows, size_t cols, cudaStream_t stream);
 
+// Block quantisation with power-of-two scales, its repetition along the other axis from 8 bits, and the way back
+// (quantize_block.cu); q / qt may be NULL together with their scales.
+int quantize_block_launch(int in_dtype, const void* in, size_t ld_in, size_t rows, size_t cols, int block_rows, void* q,
+                          size_t ld_q, uint8_t* scale, void* qt, size_t ld_qt, uint8_t* scale_t, cudaStream_t stream);
+int requantize_block_launch(const void* q, size_t ld_q, const uint8_t* scale, size_t rows, size_t cols, void* qt,
+                            size_t ld_qt, uint8_t* scale_t, cudaStream_t stream);
+int dequantize_block_launch(int out_dtype, const void* q, size_t ld_q, const uint8_t* scale, int block_rows, size_t rows,
+                            size_t cols, void* out, size_t ld_out, cudaStream_t stream);
+
 // Widens packed signed 4-bit values (two per byte, low nibble first) to int8: out[r*ld_out + c] for c < cols.
 // ld_in_elems counts 4-bit elements (even); cols even (int4.cu).
 int unpack_int4_launch(const void* in, size_t ld_in_elems, void* out, size_t ld_out, size_t rows, size_t cols,
@@ -40,6 +49,7 @@ int take_test_skip_kb();
 struct EnvSettings {
     int tile_n = 0, split_k = 0, group_m = 0, cta_pair = 0, relayout_b = 0, max_ctas = 0, direct_store = 0;
     int full_a_tile = 0, tail_split_off = 0, balance = 0, prefetch_off = 0, prefetch_force = 0, kcluster_off = 0, kcluster_pair_off = 0, kgroup = 0, early_groups = -1, one_tile_off = 0, even_runs = 0;
+    int e8m0_tile_m = 0, e8m0_slices = 0;
     int host_bands = 0, host_bands_n = 0;  // 0 = default
 };
 const EnvSettings& env_settings();

@@ -1,0 +1,285 @@
+"""Block quantisation with power-of-two scales, the 8-bit checkpoint's two ways back, and the product of such operands,
+against 64-bit references.
+
+Quantised results are compared bit for bit: the scale follows from a comparison and x * 2^-E is exact, so a code has one
+rounding, which both sides make to nearest even. The product's tolerance: the tensor core adds K/32 groups of exact products
+(two 4-bit significands) to a fp32 sum, at most one fp32 step, 2^-23, of the running magnitude lost per group and at most
+another 2^-23 where the group's products are aligned to one another; S <= 8 slices are added on top. So |error| <=
+(2 * ceil(K/32) + 8) * 2^-23 * sum |a b|, plus half a step of the output type."""
+import math
+
+import pytest
+import torch
+
+from block_reference import E4M3, E8M0, bytes_of, quantize, values
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+HALF_STEP = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
+
+
+def _data(rows, cols, dtype, dev, seed, spread=3.0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, cols, generator=g) * torch.exp2(torch.randn(rows, 1, generator=g) * spread)
+    return x.to(dtype).to(dev)
+
+
+def _check_forms(qlib, x, square, forms=("row", "column", "both")):
+    q_ref, s_ref = quantize(x, square)
+    qt_ref, st_ref = quantize(x.t(), square)
+    for form in forms:
+        out = qlib.quantize_block(x, square=square, form=form)
+        if form != "column":
+            assert torch.equal(bytes_of(out[1]), s_ref), form
+            assert torch.equal(bytes_of(out[0]), q_ref), form
+        if form != "row":
+            assert torch.equal(bytes_of(out[-1]), st_ref), form
+            assert torch.equal(bytes_of(out[-2]), qt_ref), form
+
+
+SIZES = [(1, 1), (1, 7168), (5, 16), (128, 128), (127, 129), (129, 127), (300, 520), (257, 1000), (1000, 3)]
+
+
+@pytest.mark.parametrize("rows,cols", SIZES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("square", [False, True])
+def test_quantize_block_is_exact(qlib, dev, rows, cols, dtype, square):
+    _check_forms(qlib, _data(rows, cols, dtype, dev, rows * 7 + cols), square)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("square", [False, True])
+def test_quantize_block_reads_and_writes_strided(qlib, dev, dtype, square):
+    """Odd offsets and leading dimensions on either side; what lies around the matrices stays as it was."""
+    wide = _data(260, 411, dtype, dev, 5)
+    x = wide[3:250, 7:340]  # 247 x 333, not on a vector boundary
+    rows, cols = x.shape
+    q_ref, s_ref = quantize(x, square)
+    qt_ref, st_ref = quantize(x.t(), square)
+    qb = torch.full((rows + 2, cols + 13), 0x55, dtype=torch.uint8, device=dev)
+    tb = torch.full((cols + 2, rows + 9), 0x55, dtype=torch.uint8, device=dev)
+    q, qt = qb.view(E4M3)[1:rows + 1, 5:cols + 5], tb.view(E4M3)[1:cols + 1, 3:rows + 3]
+    s = torch.empty(s_ref.shape, dtype=E8M0, device=dev)
+    st = torch.empty(st_ref.shape, dtype=E8M0, device=dev)
+    got = qlib.quantize_block(x, square=square, form="both", out=(q, s, qt, st))
+    assert got[0].data_ptr() == q.data_ptr()
+    assert torch.equal(bytes_of(q), q_ref) and torch.equal(bytes_of(s), s_ref)
+    assert torch.equal(bytes_of(qt), qt_ref) and torch.equal(bytes_of(st), st_ref)
+    for buf, view in ((qb, q), (tb, qt)):
+        view.view(torch.uint8).fill_(0x55)
+        assert bool((buf == 0x55).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("square", [False, True])
+def test_quantize_block_special_values(qlib, dev, dtype, square):
+    """Zeros, infinities, NaN, the type's largest and smallest values, and maxima on and next to 448 * 2^e."""
+    x = _data(384, 640, dtype, dev, 11, 1.0)
+    fi = torch.finfo(dtype)
+    x[0:128, 0:128] = 0
+    x[1, 130] = float("inf")
+    x[2, 260] = float("nan")
+    x[3, 390] = -float("inf")
+    x[130, 0:128] = fi.max
+    x[131, 5] = fi.smallest_normal
+    x[260:384, 128:256] = torch.finfo(dtype).tiny / 4  # subnormals
+    x[200, 256:384] = 0
+    x[200, 300] = 448.0
+    x[201, 256:384] = 0
+    x[201, 300] = 448.0 * (1 + fi.eps)
+    x[202, 256:384] = 0
+    x[202, 300] = -0.875
+    x[256:384, 512:640] = -fi.max
+    _check_forms(qlib, x, square)
+
+
+def test_quantize_block_empty(qlib, dev):
+    for rows, cols in ((0, 256), (256, 0), (0, 0)):
+        for form in ("row", "column", "both"):
+            out = qlib.quantize_block(torch.empty(rows, cols, device=dev), form=form)
+            assert out[0].shape == ((rows, cols) if form != "column" else (cols, rows))
+
+
+@pytest.mark.parametrize("rows,cols", SIZES + [(640, 384)])
+def test_requantize_block_is_exact(qlib, dev, rows, cols):
+    q, s = qlib.quantize_block(_data(rows, cols, torch.float32, dev, 3 * rows + cols, 8.0))
+    qt_ref, st_ref = quantize(values(q, s).t())
+    qt, st = qlib.requantize_block(q, s)
+    assert torch.equal(bytes_of(st), st_ref) and torch.equal(bytes_of(qt), qt_ref)
+
+
+def test_requantize_and_dequantize_every_code_and_scale(qlib, dev):
+    """All 256 codes (NaN among them) under all 256 scale bytes: rows of one scale, columns of one code, so that a
+    column's block meets 128 neighbouring scales."""
+    codes = torch.arange(256, dtype=torch.uint8).repeat(256, 1).contiguous()
+    scale = torch.arange(256, dtype=torch.uint8).repeat(2, 1).contiguous()
+    q, s = codes.to(dev).view(E4M3), scale.to(dev).view(E8M0)
+    ref = values(codes, scale)
+    qt_ref, st_ref = quantize(ref.t())
+    qt, st = qlib.requantize_block(q, s)
+    assert torch.equal(bytes_of(st), st_ref)
+    assert torch.equal(bytes_of(qt), qt_ref)
+    # single rows: each scale alone, down to 2^-127 and up to 2^127
+    for e in (0, 1, 7, 8, 9, 127, 246, 253, 254):
+        one = torch.full((2, 1), e, dtype=torch.uint8)
+        qt_ref, st_ref = quantize(values(codes[:1], one).t())
+        qt, st = qlib.requantize_block(q[:1], one.to(dev).view(E8M0))
+        assert torch.equal(bytes_of(st), st_ref), e
+        assert torch.equal(bytes_of(qt), qt_ref), e
+    for dtype in TYPES:
+        got = qlib.dequantize_block(q, s, dtype).cpu()
+        want = ref.to(torch.float32).to(dtype)  # the first step is exact, or overflows as the second would
+        assert torch.equal(torch.isnan(got), torch.isnan(want))
+        ok = ~torch.isnan(want)
+        assert torch.equal(got[ok], want[ok])
+
+
+@pytest.mark.parametrize("rows,cols", SIZES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("square", [False, True])
+def test_dequantize_block_is_exact(qlib, dev, rows, cols, dtype, square):
+    q, s = qlib.quantize_block(_data(rows, cols, torch.float32, dev, rows + cols), square=square)
+    got = qlib.dequantize_block(q, s, dtype)
+    assert torch.equal(got.cpu(), values(q, s).to(torch.float32).to(dtype))
+    buf = torch.full((rows, cols + 5), 7.0, dtype=dtype, device=dev)
+    qlib.dequantize_block(q, s, out=buf[:, 3:cols + 3])
+    assert torch.equal(buf[:, 3:cols + 3], got)
+    assert bool((buf[:, :3] == 7).all()) and bool((buf[:, cols + 3:] == 7).all())
+
+
+# ------------------------------------------------------------------------------------------------ the product
+def _operands(qlib, dev, M, N, K, a_square, b_square, seed, spread=2.0):
+    a, sa = qlib.quantize_block(_data(M, K, torch.float32, dev, seed, spread), square=a_square)
+    b, sb = qlib.quantize_block(_data(N, K, torch.float32, dev, seed + 1, spread), square=b_square)
+    return a, sa, b, sb
+
+
+def _product(a, sa, b, sb):
+    """(reference, sum of magnitudes) in 64 bits, on the GPU for speed."""
+    av, bv = values(a, sa).to(a.device), values(b, sb).to(a.device)
+    return (av @ bv.t()), (av.abs() @ bv.abs().t())
+
+
+def _assert_close(got, ref, mags, K, dtype):
+    tol = (2 * math.ceil(K / 32) + 8) * 2.0 ** -23 * mags + HALF_STEP[dtype] * ref.abs() * (1 + 2.0 ** -7)
+    if dtype == torch.float16:
+        tol = tol + 2.0 ** -25  # half a step of its subnormals
+    err = (got.double() - ref).abs()
+    worst = float((err - tol).max())
+    assert worst <= 0, f"error {float(err.max())} exceeds its bound by {worst}"
+
+
+PRODUCTS = [(1, 128, 128), (1, 7168, 2048), (2, 1, 1), (3, 17, 129), (16, 256, 640), (17, 520, 384), (33, 1000, 1040),
+            (64, 2048, 4096), (100, 200, 520), (128, 384, 256), (130, 77, 256), (300, 520, 1040), (520, 1100, 1536),
+            (1024, 2048, 640), (2100, 2300, 900)]
+
+
+@pytest.mark.parametrize("M,N,K", PRODUCTS)
+@pytest.mark.parametrize("out", TYPES)
+@pytest.mark.parametrize("a_square,b_square", [(False, True), (False, False), (True, False)])
+def test_product_matches_64_bits(qlib, dev, M, N, K, out, a_square, b_square):
+    a, sa, b, sb = _operands(qlib, dev, M, N, K, a_square, b_square, M + N + K)
+    ref, mags = _product(a, sa, b, sb)
+    if out == torch.float16:  # keep within its range: scaled down exactly, by a power of two
+        down = 2.0 ** math.ceil(math.log2(max(float(ref.abs().max()), 1.0) / 2.0 ** 14))
+        sa = (sa.view(torch.uint8) - int(math.log2(down))).view(E8M0)
+        ref, mags = ref / down, mags / down
+    c = torch.full((M, N), float("nan"), dtype=out, device=dev)
+    qlib.fp8_block_mm_e8m0(a, b, sa, sb, c)
+    _assert_close(c, ref, mags, K, out)
+    again = torch.zeros_like(c)
+    qlib.fp8_block_mm_e8m0(a, b, sa, sb, again)
+    assert torch.equal(c, again)
+    rc, st = qlib.device_status()
+    assert rc == 0, st
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 300, 384), (64, 2048, 1000), (300, 520, 1040), (777, 2048, 4001), (2304, 2176, 384)])
+def test_product_accumulates(qlib, dev, M, N, K):
+    a, sa, b, sb = _operands(qlib, dev, M, N, K, False, False, M + N)
+    ref, mags = _product(a, sa, b, sb)
+    old = torch.randn(M, N, device=dev) * float(ref.abs().mean())
+    c = old.clone()
+    qlib.fp8_block_mm_e8m0(a, b, sa, sb, c, accumulate=True)
+    _assert_close(c, ref + old.double(), mags + old.abs().double(), K, torch.float32)
+    wide = torch.full((M, N + 7), 3.0, device=dev)  # no vector boundary anywhere, and neighbours to leave alone
+    c = wide[:, 3:N + 3]
+    c.copy_(old)
+    qlib.fp8_block_mm_e8m0(a, b, sa, sb, c, accumulate=True)
+    _assert_close(c, ref + old.double(), mags + old.abs().double(), K, torch.float32)
+    assert bool((wide[:, :3] == 3).all()) and bool((wide[:, N + 3:] == 3).all())
+
+
+@pytest.mark.parametrize("M,N,K", [(5, 300, 384), (300, 520, 1040), (2100, 2300, 256)])
+@pytest.mark.parametrize("out", TYPES)
+def test_product_strided(qlib, dev, M, N, K, out):
+    """Operands cut out of wider matrices, C at an odd offset."""
+    a, sa, b, sb = _operands(qlib, dev, M, N, K, False, True, 3)
+    wa = torch.zeros(M + 1, (K // 16 + 4) * 16, dtype=torch.uint8, device=dev).view(E4M3)
+    wb = torch.zeros(N + 1, (K // 16 + 5) * 16, dtype=torch.uint8, device=dev).view(E4M3)
+    wa.view(torch.uint8).fill_(0x7F)  # NaN all around
+    wb.view(torch.uint8).fill_(0x7F)
+    va, vb = wa[1:, 16:16 + K], wb[1:, 32:32 + K]
+    va.view(torch.uint8).copy_(a.view(torch.uint8))
+    vb.view(torch.uint8).copy_(b.view(torch.uint8))
+    wide = torch.full((M + 2, N + 7), 3.0, dtype=out, device=dev)
+    c = wide[1:M + 1, 5:N + 5]
+    down = 2.0 ** 20 if out == torch.float16 else 1.0
+    sa = (sa.view(torch.uint8) - int(math.log2(down))).view(E8M0)
+    qlib.fp8_block_mm_e8m0(va, vb, sa, sb, c)
+    ref, mags = _product(a, sa, b, sb)
+    _assert_close(c, ref, mags, K, out)
+    c.fill_(3.0)
+    assert bool((wide == 3).all())
+
+
+def test_product_scales_far_apart(qlib, dev):
+    """Scale bytes over the whole range whose products cancel out, one element of each K block at a time."""
+    M, N, K = 130, 140, 1024
+    a = torch.zeros(M, K, dtype=torch.uint8)
+    b = torch.zeros(N, K, dtype=torch.uint8)
+    g = torch.Generator().manual_seed(2)
+    kb = K // 128
+    at = torch.randint(0, 128, (kb,), generator=g) + torch.arange(kb) * 128
+    a[:, at] = torch.randint(8, 120, (M, kb), generator=g, dtype=torch.uint8)
+    b[:, at] = torch.randint(8, 120, (N, kb), generator=g, dtype=torch.uint8)
+    ea = torch.randint(1, 254, (kb, 1), generator=g)
+    sa = (ea + torch.zeros(kb, M, dtype=torch.int64)).to(torch.uint8)
+    sb = (254 - ea + torch.randint(-3, 4, (kb, N), generator=g)).clamp(1, 254).to(torch.uint8)
+    a, b, sa, sb = a.to(dev).view(E4M3), b.to(dev).view(E4M3), sa.to(dev).view(E8M0), sb.to(dev).view(E8M0)
+    ref, mags = _product(a, sa, b, sb)
+    c = torch.empty(M, N, device=dev)
+    qlib.fp8_block_mm_e8m0(a, b, sa, sb, c)
+    _assert_close(c, ref, mags, K, torch.float32)
+
+
+def test_product_nan_blocks_reach_their_rows_only(qlib, dev):
+    x = _data(200, 512, torch.bfloat16, dev, 1, 1.0)
+    w = _data(300, 512, torch.bfloat16, dev, 2, 1.0)
+    x[7, 130] = float("inf")
+    w[250, 400] = float("nan")
+    a, sa = qlib.quantize_block(x)
+    b, sb = qlib.quantize_block(w)
+    c = torch.empty(200, 300, device=dev)
+    qlib.fp8_block_mm_e8m0(a, b, sa, sb, c)
+    bad = torch.zeros(200, 300, dtype=torch.bool, device=dev)
+    bad[7], bad[:, 250] = True, True
+    assert torch.equal(torch.isnan(c), bad)
+    # a NaN scale over finite codes
+    sb2 = sb.view(torch.uint8).clone()
+    sb2[1, 3] = 255
+    qlib.fp8_block_mm_e8m0(a, b, sa, sb2.view(E8M0), c)
+    bad[:, 3] = True
+    assert torch.equal(torch.isnan(c), bad)
+
+
+def test_product_empty(qlib, dev):
+    e = lambda r, c: qlib.quantize_block(torch.ones(r, c, device=dev))  # noqa: E731
+    for M, N, K in ((0, 128, 128), (128, 0, 128), (5, 7, 0)):
+        (a, sa), (b, sb) = e(M, K), e(N, K)
+        c = torch.full((M, N), 3.0, device=dev)
+        qlib.fp8_block_mm_e8m0(a, b, sa, sb, c, accumulate=True)
+        assert bool((c == 3).all())
+        qlib.fp8_block_mm_e8m0(a, b, sa, sb, c)
+        assert bool((c == 0).all())
