@@ -944,8 +944,13 @@ E8m0Plan plan_e8m0(size_t M, size_t N, int kb_total, int sms) {
     const long long tiles = static_cast<long long>((M + pl.tile_m - 1) / pl.tile_m) * static_cast<long long>((N + 127) / 128);
     pl.slices = 1;
     while (pl.slices < 8 && tiles * pl.slices * 2 <= 2ll * sms && kb_total >= pl.slices * 2) pl.slices *= 2;
-    if (g_env.e8m0_tile_m > 0) pl.tile_m = g_env.e8m0_tile_m;
-    if (g_env.e8m0_slices > 0) pl.slices = std::min(g_env.e8m0_slices, kb_total);
+    if (M > 512 && N > 512) pl = {256, 256, 1};
+    if (g_env.e8m0_tile_m > 0) {
+        pl.tile_m = g_env.e8m0_tile_m;
+        pl.tile_n = pl.tile_m == 256 ? 256 : 128;
+        pl.slices = 1;
+    }
+    if (g_env.e8m0_slices > 0 && pl.tile_m != 256 && g_env.e8m0_slices <= kb_total) pl.slices = g_env.e8m0_slices;
     return pl;
 }
 
@@ -1078,14 +1083,26 @@ int e8m0_dispatch(int out_dtype, const void* A, size_t lda, const uint8_t* a_sca
     p.c_vec_ok = reinterpret_cast<uintptr_t>(C) % (4 * out_bytes) == 0 && ldc % 4 == 0;
 
     const E8m0Plan plan = plan_e8m0(M, N, p.kb_total, st->sm_count);
-    CUtensorMap ta, tb;
+    CUtensorMap ta, tb, tc;
     p.m_tiles = static_cast<int>((M + plan.tile_m - 1) / plan.tile_m);
     p.n_tiles = static_cast<int>((N + plan.tile_n - 1) / plan.tile_n);
     if (static_cast<long long>(p.m_tiles) * p.n_tiles * 8 > 0x7fffffffLL) return QGEMM_ERR_UNSUPPORTED;
-    rc = make_operand_map(A, M, K, lda, QGEMM_DTYPE_FP8_E4M3, static_cast<uint32_t>(plan.tile_m), &ta);
+    rc = make_operand_map(A, M, K, lda, QGEMM_DTYPE_FP8_E4M3, static_cast<uint32_t>(std::min(plan.tile_m, 128)), &ta);
     if (rc != QGEMM_OK) return rc;
     rc = make_operand_map(B, N, K, ldb, QGEMM_DTYPE_FP8_E4M3, 128u, &tb);
     if (rc != QGEMM_OK) return rc;
+    if (plan.tile_m == 256) {  // CTA pairs
+        std::memset(&tc, 0, sizeof(tc));
+        if (reinterpret_cast<uintptr_t>(C) % 16 == 0 && (ldc * out_bytes) % 16 == 0 && g_env.direct_store == 0)
+            p.c_tma_ok = make_output_map(C, M, N, ldc, 1, out_kind, &tc) == QGEMM_OK ? 1 : 0;
+        // tile rows walked together, so that their panels of A (16 MB of them) stay in L2 while B passes
+        p.group_m = g_env.group_m > 0
+                        ? g_env.group_m
+                        : static_cast<int>(std::max<long long>(4, std::min<long long>(4096, (16ll << 20) / (128ll * p.kb_total * 256))));
+        p.idesc = ptx::make_idesc_e8m0(256u, 256u);
+        const int clusters = static_cast<int>(std::min<long long>(static_cast<long long>(p.m_tiles) * p.n_tiles, st->sm_count / 2));
+        return launch_e8m0_pair(ta, tb, tc, p, clusters, stream) == cudaSuccess ? QGEMM_OK : QGEMM_ERR_CUDA;
+    }
     p.idesc = ptx::make_idesc_e8m0(128u, static_cast<uint32_t>(plan.tile_m));
     return launch_e8m0_small(plan.tile_m, plan.slices, ta, tb, p, stream) == cudaSuccess ? QGEMM_OK : QGEMM_ERR_CUDA;
 }

@@ -54,7 +54,36 @@ cudaError_t launch_small(int slices, const CUtensorMap& ta, const CUtensorMap& t
     }
 }
 
+template <int OUT>
+cudaError_t launch_pair_one(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const E8m0Params& p,
+                            int clusters, cudaStream_t stream) {
+    auto kernel = gemm_e8m0_pair_kernel<OUT>;
+    constexpr int smem = E8PairSmem::kDynamicBytes;
+    static_assert(smem <= 227 * 1024, "dynamic shared memory of one CTA");
+    static bool configured[64] = {};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (!configured[dev]) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return e;
+        configured[dev] = true;
+    }
+    return launch_pdl(kernel, dim3(2 * clusters), dim3(kE8Threads), smem, stream, ta, tb, tc, p);
+}
+
 }  // namespace
+
+cudaError_t launch_e8m0_pair(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const E8m0Params& p,
+                             int clusters, cudaStream_t stream) {
+    switch (p.out) {
+        case OUT_F32: return launch_pair_one<OUT_F32>(ta, tb, tc, p, clusters, stream);
+        case OUT_BF16: return launch_pair_one<OUT_BF16>(ta, tb, tc, p, clusters, stream);
+        case OUT_F16: return launch_pair_one<OUT_F16>(ta, tb, tc, p, clusters, stream);
+        default: return cudaErrorInvalidValue;
+    }
+}
 
 cudaError_t launch_e8m0_small(int tokens_per_tile, int slices, const CUtensorMap& ta, const CUtensorMap& tb,
                               const E8m0Params& p, cudaStream_t stream) {

@@ -380,8 +380,328 @@ gemm_e8m0_small_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
     }
 }
 
+// ==================================================================================== large products
+// CTA pairs on 256 x 256 tiles (tcgen05.mma.cta_group::2; the ring, the pair's barriers and the persistent tile loop as in
+// gemm_sm100_2cta.cuh). Each CTA's tensor memory has 512 columns: two 256-column accumulators would leave none for scales,
+// so the second accumulator starts at column 192 and the last 64 columns hold four chunks of scales. The accumulators
+// share columns 192..255: the epilogue drains those first and hands them over (`ovl`), and the next tile's MMAs run under
+// the rest of the drain. The first instruction of a tile waits only for a quarter of its predecessor's epilogue.
+//
+// Scales: the leader's instruction multiplies each CTA's 128 rows by that CTA's A scales, and all 256 columns by the B
+// scales, which both CTAs hold in full; the scale warps of either CTA write their own shared memory and arrive on the
+// leader's `sfull`; one tcgen05.cp of the leader copies in both CTAs.
+struct E8PairSmem {
+    static constexpr int kBN = 256;
+    static constexpr int kStages = 6;
+    static constexpr int kAStage = 128 * 128;
+    static constexpr int kBStage = (kBN / 2) * 128;
+    static constexpr int kTiles = kStages * (kAStage + kBStage);
+    static constexpr int kOutOffset = kTiles;  // one 4 KB staging box per epilogue warp
+    static constexpr int kScaleOffset = kOutOffset + 4 * 4096;
+    static constexpr int kScaleSlot = 512 + (kBN / 128) * 512;  // this CTA's 128 rows of A, all rows of B
+    static constexpr int kBarOffset = kScaleOffset + kE8Slots * kScaleSlot;
+    static constexpr int kBars = 2 * kStages + 2 * kE8Slots + 3;  // full, empty, sfull, sempty, tfull[2], ovl
+    static constexpr int kMiscOffset = kBarOffset + kBars * 8;
+    static constexpr int kTotal = kMiscOffset + 16;
+    static constexpr int kDynamicBytes = kTotal + 1024;
+    static constexpr uint32_t kAccStep = 192;   // first column of the second accumulator
+    static constexpr uint32_t kScaleCol = 448;  // first column of the scales
+    static constexpr uint32_t kScaleCols = 4 + kBN / 32;  // columns of a chunk: A's, then B's
+    static_assert(kAccStep + kBN <= kScaleCol && kScaleCol + kE8Slots * kScaleCols <= 512, "tensor-memory columns");
+};
+
+template <int OUT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kE8Threads, 1)
+gemm_e8m0_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+                      const __grid_constant__ CUtensorMap tmap_c, const E8m0Params p) {
+    using L = E8PairSmem;
+    constexpr int STAGES = L::kStages, BN = L::kBN;
+    constexpr int OB = OutBytes<OUT>::value;
+    constexpr int CW = 128 / OB;  // columns of a staged box: 64 (16-bit out) or 32
+
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw_addr = ptx::smem_u32(smem_raw);
+    const uint32_t pad = ((raw_addr + 1023u) & ~1023u) - raw_addr;
+    uint8_t* smem = smem_raw + pad;
+    const uint32_t smem_base = raw_addr + pad;
+    const uint32_t smem_a = smem_base;
+    const uint32_t smem_b = smem_base + STAGES * L::kAStage;
+    const uint32_t smem_s = smem_base + L::kScaleOffset;
+    const uint32_t bar_full = smem_base + L::kBarOffset;
+    const uint32_t bar_empty = bar_full + STAGES * 8;
+    const uint32_t bar_sfull = bar_empty + STAGES * 8;
+    const uint32_t bar_sempty = bar_sfull + kE8Slots * 8;
+    const uint32_t bar_tfull = bar_sempty + kE8Slots * 8;
+    const uint32_t bar_ovl = bar_tfull + 2 * 8;
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + L::kMiscOffset);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMiscOffset + 4);
+
+    const int warp = static_cast<int>(threadIdx.x) >> 5;
+    const int lane = static_cast<int>(threadIdx.x) & 31;
+    const uint32_t rank = ptx::cluster_ctarank();  // 0 = leader
+    const int cluster_id = static_cast<int>(blockIdx.x) >> 1;
+    const int n_clusters = static_cast<int>(gridDim.x) >> 1;
+    const int total_work = p.m_tiles * p.n_tiles;
+    const uint32_t peer_abort = ptx::mapa_shared(ptx::smem_u32(const_cast<int*>(abort_flag)), rank ^ 1u);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            ptx::mbar_init(bar_full + s * 8, 1);
+            ptx::mbar_init(bar_empty + s * 8, 1);
+        }
+        for (int s = 0; s < kE8Slots; ++s) {
+            ptx::mbar_init(bar_sfull + s * 8, 4);  // two scale warps of each CTA
+            ptx::mbar_init(bar_sempty + s * 8, 1);
+        }
+        ptx::mbar_init(bar_tfull, 1);
+        ptx::mbar_init(bar_tfull + 8, 1);
+        ptx::mbar_init(bar_ovl, 8);  // four epilogue warps of each CTA
+        *abort_flag = 0;
+        ptx::fence_barrier_init();
+    }
+    if (warp == 0 && lane == 0) {
+        ptx::prefetch_tensormap(&tmap_a);
+        ptx::prefetch_tensormap(&tmap_b);
+        if (p.c_tma_ok) ptx::prefetch_tensormap(&tmap_c);
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc_pair(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
+        ptx::tmem_relinquish_pair();
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::cluster_arrive();
+    ptx::cluster_wait();
+    ptx::tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    ptx::pdl_launch_dependents();
+    ptx::pdl_wait();
+
+    if (warp == 0) {
+        // ------------------------------------------------------------ TMA producer (both CTAs)
+        if (ptx::elect_one()) {
+            uint32_t stage = 0, phase = 0;
+            bool ok = true;
+            for (int w = cluster_id; ok && w < total_work; w += n_clusters) {
+                int m_blk, n_blk;
+                e8_decode(w, p, m_blk, n_blk);
+                const int row_a = (m_blk * 2 + static_cast<int>(rank)) * 128;
+                const int row_b = n_blk * BN + static_cast<int>(rank) * (BN / 2);
+                for (int kb = 0; kb < p.kb_total; ++kb) {
+                    if (!wait_bounded(bar_empty + stage * 8, phase ^ 1u, abort_flag, p.status, ROLE_PRODUCER, kb, peer_abort)) {
+                        ok = false;
+                        break;
+                    }
+                    if (rank == 0) ptx::mbar_arrive_expect_tx(bar_full + stage * 8, 2 * (L::kAStage + L::kBStage));
+                    const uint32_t leader_full = ptx::mapa_shared(bar_full + stage * 8, 0);
+                    ptx::tma_load_2d_pair(smem_a + stage * L::kAStage, &tmap_a, leader_full, kb * 128, row_a);
+                    ptx::tma_load_2d_pair(smem_b + stage * L::kBStage, &tmap_b, leader_full, kb * 128, row_b);
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------------------ MMA issuer (leader CTA only)
+        if (rank == 0 && ptx::elect_one()) {
+            uint32_t stage = 0, phase = 0, slot = 0, sphase = 0;
+            uint32_t it = 0;
+            bool ok = true;
+            for (int w = cluster_id; ok && w < total_work; w += n_clusters, ++it) {
+                const uint32_t acc = it & 1u;
+                const uint32_t d_tmem = tmem_base + acc * L::kAccStep;
+                // the previous tile's share of the common columns is out (and with it everything of the tile before)
+                if (it > 0 && !wait_bounded(bar_ovl, (it - 1) & 1u, abort_flag, p.status, ROLE_MMA, -1, peer_abort)) break;
+                for (int kc = 0; ok && kc < p.kb_total; kc += 4) {
+                    if (!wait_bounded_cluster(bar_sfull + slot * 8, sphase, abort_flag, p.status, ROLE_MMA, -2 - kc, peer_abort)) {
+                        ok = false;
+                        break;
+                    }
+                    ptx::tc_fence_after();
+                    const uint32_t sa_tmem = tmem_base + L::kScaleCol + slot * L::kScaleCols, sb_tmem = sa_tmem + 4;
+                    const uint32_t src = smem_s + slot * L::kScaleSlot;
+                    ptx::tc_copy_scales_pair(sa_tmem, ptx::make_scale_desc(src));
+#pragma unroll
+                    for (int h = 0; h < BN / 128; ++h)
+                        ptx::tc_copy_scales_pair(sb_tmem + 4 * h, ptx::make_scale_desc(src + 512 + 512 * h));
+                    const int n = min(4, p.kb_total - kc);
+                    for (int i = 0; i < n; ++i) {
+                        if (!wait_bounded(bar_full + stage * 8, phase, abort_flag, p.status, ROLE_MMA, kc + i, peer_abort)) {
+                            ok = false;
+                            break;
+                        }
+                        ptx::tc_fence_after();
+                        const uint64_t a_desc = ptx::make_kmajor_sw128_desc(smem_a + stage * L::kAStage);
+                        const uint64_t b_desc = ptx::make_kmajor_sw128_desc(smem_b + stage * L::kBStage);
+                        const uint32_t idesc = p.idesc | ptx::idesc_scale_id(static_cast<uint32_t>(i));
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            ptx::umma_e8m0_pair(d_tmem, a_desc + 2u * k, b_desc + 2u * k, idesc, sa_tmem, sb_tmem,
+                                                (kc + i > 0 || k > 0) ? 1u : 0u);
+                        ptx::tc_commit_pair(bar_empty + stage * 8, 3);
+                        if (++stage == STAGES) {
+                            stage = 0;
+                            phase ^= 1u;
+                        }
+                    }
+                    if (!ok) break;
+                    ptx::tc_commit_pair(bar_sempty + slot * 8, 3);
+                    if (++slot == kE8Slots) {
+                        slot = 0;
+                        sphase ^= 1u;
+                    }
+                }
+                if (ok) ptx::tc_commit_pair(bar_tfull + acc * 8, 3);
+            }
+        }
+    } else if (warp >= 6) {
+        // ------------------------------------------------------------ scales (both CTAs): warp 6 A's, warp 7 B's
+        const bool of_a = warp == 6;
+        uint32_t slot = 0, sphase = 1;  // the first pass over the slots finds them free
+        bool ok = true;
+        for (int w = cluster_id; ok && w < total_work; w += n_clusters) {
+            int m_blk, n_blk;
+            e8_decode(w, p, m_blk, n_blk);
+            const int row_a = (m_blk * 2 + static_cast<int>(rank)) * 128, row_b = n_blk * BN;
+            for (int kc = 0; kc < p.kb_total; kc += 4) {
+                const int n = min(4, p.kb_total - kc);
+                uint4 v[BN / 128];
+                if (of_a) {
+                    v[0] = gather_scales(p.a_scale, p.a_rows, p.a_shift, row_a, p.M, kc, n, lane);
+                } else {
+#pragma unroll
+                    for (int h = 0; h < BN / 128; ++h)
+                        v[h] = gather_scales(p.b_scale, p.b_rows, p.b_shift, row_b + 128 * h, p.N, kc, n, lane);
+                }
+                if (!wait_bounded(bar_sempty + slot * 8, sphase, abort_flag, p.status, ROLE_SCALES, kc, peer_abort)) {
+                    ok = false;
+                    break;
+                }
+                const uint32_t dst = smem_s + slot * L::kScaleSlot + lane * 16;
+                if (of_a) {
+                    ptx::st_shared_v4(dst, v[0].x, v[0].y, v[0].z, v[0].w);
+                } else {
+#pragma unroll
+                    for (int h = 0; h < BN / 128; ++h)
+                        ptx::st_shared_v4(dst + 512 + 512 * h, v[h].x, v[h].y, v[h].z, v[h].w);
+                }
+                ptx::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive_cluster(ptx::mapa_shared(bar_sfull + slot * 8, 0));
+                if (++slot == kE8Slots) {
+                    slot = 0;
+                    sphase ^= 1u;
+                }
+            }
+        }
+    } else {
+        // ------------------------------------------------------------ epilogue (both CTAs)
+        const int quad = warp & 3;
+        const uint32_t stage_base = smem_base + L::kOutOffset + quad * 4096u;
+        uint32_t it = 0;
+        for (int w = cluster_id; w < total_work; w += n_clusters, ++it) {
+            int m_blk, n_blk;
+            e8_decode(w, p, m_blk, n_blk);
+            const uint32_t acc = it & 1u;
+            if (!wait_bounded(bar_tfull + acc * 8, (it >> 1) & 1u, abort_flag, p.status, ROLE_EPILOGUE, w, peer_abort)) break;
+            ptx::tc_fence_after();
+            const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * L::kAccStep;
+            const int row0 = (m_blk * 2 + static_cast<int>(rank)) * 128 + quad * 32;
+            // the columns that both accumulators use come first: the last 64 of the first, the first 64 of the second
+            const int first = acc == 0 ? static_cast<int>(L::kAccStep) / CW : 0;
+            constexpr int kShared = (BN - static_cast<int>(L::kAccStep)) / CW;  // boxes they make up
+#pragma unroll 1
+            for (int b = 0; b < BN / CW; ++b) {
+                const int c = (first + b) & (BN / CW - 1);
+                const int n0 = n_blk * BN + c * CW;
+                const bool live = row0 < p.M && n0 < p.N;  // warp-uniform
+                uint32_t v[CW];
+                if (live) {
+                    ptx::tmem_ld_32x32b_x32(t_addr + c * CW, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
+                    if constexpr (CW == 64)
+                        ptx::tmem_ld_32x32b_x32(t_addr + c * CW + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
+                    ptx::tmem_ld_wait();
+                }
+                if (b == kShared - 1) {
+                    ptx::tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive_cluster(ptx::mapa_shared(bar_ovl, 0));
+                }
+                if (!live) continue;
+                uint32_t u[32];
+                if constexpr (OUT == OUT_F32) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) u[j] = v[j];
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        if constexpr (OUT == OUT_BF16) {
+                            const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+                            u[j] = *reinterpret_cast<const uint32_t*>(&h);
+                        } else {
+                            const __half2 h = __floats2half2_rn(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+                            u[j] = *reinterpret_cast<const uint32_t*>(&h);
+                        }
+                    }
+                }
+                if (p.c_tma_ok) {
+                    // the box is free once the store before has read it
+                    if (ptx::elect_one()) ptx::tma_store_wait_read<0>();
+                    __syncwarp();
+                    const uint32_t row_addr = stage_base + static_cast<uint32_t>(lane) * 128u;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        ptx::st_shared_v4(row_addr + static_cast<uint32_t>((j ^ (lane & 7)) * 16), u[4 * j], u[4 * j + 1],
+                                          u[4 * j + 2], u[4 * j + 3]);
+                    ptx::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (ptx::elect_one()) {
+                        if (OUT == OUT_F32 && p.accumulate) ptx::tma_add_3d(&tmap_c, stage_base, n0, row0, 0);
+                        else ptx::tma_store_3d(&tmap_c, stage_base, n0, row0, 0);
+                        ptx::tma_store_commit();
+                    }
+                } else if (row0 + lane < p.M) {
+                    uint8_t* dst = static_cast<uint8_t*>(p.C) + (static_cast<long long>(row0 + lane) * p.ldc + n0) * OB;
+#pragma unroll
+                    for (int j = 0; j < CW; ++j) {
+                        if (n0 + j < p.N) {
+                            if constexpr (OUT == OUT_F32) {
+                                float* f = reinterpret_cast<float*>(dst) + j;
+                                *f = p.accumulate ? *f + __uint_as_float(u[j]) : __uint_as_float(u[j]);
+                            } else {
+                                reinterpret_cast<uint16_t*>(dst)[j] =
+                                    static_cast<uint16_t>((j & 1) ? (u[j >> 1] >> 16) : (u[j >> 1] & 0xffffu));
+                            }
+                        }
+                    }
+                }
+            }
+        }
+        if (lane == 0) ptx::tma_store_wait_read<0>();
+    }
+
+    // ---------------------------------------------------------------- teardown
+    ptx::tc_fence_before();
+    __syncthreads();
+    // neither CTA may release its shared or tensor memory while the other can still touch it
+    ptx::cluster_arrive();
+    ptx::cluster_wait();
+    if (*abort_flag != 0) {
+        for (int i = 0; i < 64; ++i) __nanosleep(20000);
+        __syncthreads();
+    }
+    if (warp == 1) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc_pair(tmem_base, 512);
+    }
+}
+
 // tokens_per_tile: 16, 32, 64 or 128; slices: 1, 2, 4 or 8, at most kb_total (gemm_e8m0.cu).
 cudaError_t launch_e8m0_small(int tokens_per_tile, int slices, const CUtensorMap& ta, const CUtensorMap& tb,
                               const E8m0Params& p, cudaStream_t stream);
+cudaError_t launch_e8m0_pair(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const E8m0Params& p,
+                             int clusters, cudaStream_t stream);
 
 }  // namespace qgemm
