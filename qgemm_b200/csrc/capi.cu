@@ -1077,6 +1077,8 @@ int e8m0_dispatch(int out_dtype, const void* A, size_t lda, const uint8_t* a_sca
     p.b_shift = b_block_rows == 128 ? 7 : 0;
     p.a_rows = static_cast<long long>(a_block_rows == 128 ? (M + 127) / 128 : M);
     p.b_rows = static_cast<long long>(b_block_rows == 128 ? (N + 127) / 128 : N);
+    p.a_words = reinterpret_cast<uintptr_t>(a_scale) % 4 == 0 && p.a_rows % 4 == 0;
+    p.b_words = reinterpret_cast<uintptr_t>(b_scale) % 4 == 0 && p.b_rows % 4 == 0;
     p.out = out_kind;
     p.accumulate = accumulate != 0;
     p.status = st->status;

@@ -70,7 +70,7 @@ cudaError_t launch_pair_one(const CUtensorMap& ta, const CUtensorMap& tb, const 
         if (e != cudaSuccess) return e;
         configured[dev] = true;
     }
-    return launch_pdl(kernel, dim3(2 * clusters), dim3(kE8Threads), smem, stream, ta, tb, tc, p);
+    return launch_pdl(kernel, dim3(2 * clusters), dim3(kE8PairThreads), smem, stream, ta, tb, tc, p);
 }
 
 }  // namespace
