@@ -236,6 +236,7 @@ EnvSettings read_env() {
     e.one_tile_off = (ot != nullptr && ot[0] == '0') ? 1 : 0;
     e.kgroup = std::max(0, env_int("QGEMM_KGROUP"));  // 0 = the library's choice, 1 = off, 2 / 4 / 8 = K blocks per load
     e.e8m0_tile_m = std::max(0, env_int("QGEMM_E8M0_TILE_M"));  // tile rows of the power-of-two block-scaled GEMM
+    e.e8m0_tile_n = std::max(0, env_int("QGEMM_E8M0_TILE_N"));
     e.e8m0_slices = std::max(0, env_int("QGEMM_E8M0_SLICES"));  // its K slices
     e.host_bands = std::max(0, env_int("QGEMM_HOST_BANDS"));
     e.host_bands_n = std::max(0, env_int("QGEMM_HOST_BANDS_N"));
@@ -950,7 +951,8 @@ E8m0Plan plan_e8m0(size_t M, size_t N, int kb_total, int sms) {
         pl.tile_n = pl.tile_m == 256 ? 256 : 128;
         pl.slices = 1;
     }
-    if (g_env.e8m0_slices > 0 && pl.tile_m != 256 && g_env.e8m0_slices <= kb_total) pl.slices = g_env.e8m0_slices;
+    if (pl.tile_m == 256 && g_env.e8m0_tile_n > 0) pl.tile_n = g_env.e8m0_tile_n;
+    if (g_env.e8m0_slices > 0 && g_env.e8m0_slices <= kb_total) pl.slices = g_env.e8m0_slices;
     return pl;
 }
 
@@ -1077,8 +1079,6 @@ int e8m0_dispatch(int out_dtype, const void* A, size_t lda, const uint8_t* a_sca
     p.b_shift = b_block_rows == 128 ? 7 : 0;
     p.a_rows = static_cast<long long>(a_block_rows == 128 ? (M + 127) / 128 : M);
     p.b_rows = static_cast<long long>(b_block_rows == 128 ? (N + 127) / 128 : N);
-    p.a_words = reinterpret_cast<uintptr_t>(a_scale) % 4 == 0 && p.a_rows % 4 == 0;
-    p.b_words = reinterpret_cast<uintptr_t>(b_scale) % 4 == 0 && p.b_rows % 4 == 0;
     p.out = out_kind;
     p.accumulate = accumulate != 0;
     p.status = st->status;
@@ -1091,7 +1091,8 @@ int e8m0_dispatch(int out_dtype, const void* A, size_t lda, const uint8_t* a_sca
     if (static_cast<long long>(p.m_tiles) * p.n_tiles * 8 > 0x7fffffffLL) return QGEMM_ERR_UNSUPPORTED;
     rc = make_operand_map(A, M, K, lda, QGEMM_DTYPE_FP8_E4M3, static_cast<uint32_t>(std::min(plan.tile_m, 128)), &ta);
     if (rc != QGEMM_OK) return rc;
-    rc = make_operand_map(B, N, K, ldb, QGEMM_DTYPE_FP8_E4M3, 128u, &tb);
+    const uint32_t b_box = plan.tile_m == 256 ? static_cast<uint32_t>(plan.tile_n / 2) : 128u;  // a pair's CTAs load half each
+    rc = make_operand_map(B, N, K, ldb, QGEMM_DTYPE_FP8_E4M3, b_box, &tb);
     if (rc != QGEMM_OK) return rc;
     if (plan.tile_m == 256) {  // CTA pairs
         std::memset(&tc, 0, sizeof(tc));
@@ -1101,9 +1102,9 @@ int e8m0_dispatch(int out_dtype, const void* A, size_t lda, const uint8_t* a_sca
         p.group_m = g_env.group_m > 0
                         ? g_env.group_m
                         : static_cast<int>(std::max<long long>(4, std::min<long long>(4096, (16ll << 20) / (128ll * p.kb_total * 256))));
-        p.idesc = ptx::make_idesc_e8m0(256u, 256u);
+        p.idesc = ptx::make_idesc_e8m0(256u, static_cast<uint32_t>(plan.tile_n));
         const int clusters = static_cast<int>(std::min<long long>(static_cast<long long>(p.m_tiles) * p.n_tiles, st->sm_count / 2));
-        return launch_e8m0_pair(ta, tb, tc, p, clusters, stream) == cudaSuccess ? QGEMM_OK : QGEMM_ERR_CUDA;
+        return launch_e8m0_pair(plan.tile_n, plan.slices, ta, tb, tc, p, clusters, stream) == cudaSuccess ? QGEMM_OK : QGEMM_ERR_CUDA;
     }
     p.idesc = ptx::make_idesc_e8m0(128u, static_cast<uint32_t>(plan.tile_m));
     return launch_e8m0_small(plan.tile_m, plan.slices, ta, tb, p, stream) == cudaSuccess ? QGEMM_OK : QGEMM_ERR_CUDA;

@@ -195,6 +195,37 @@ def test_product_matches_64_bits(qlib, dev, M, N, K, out, a_square, b_square):
     assert rc == 0, st
 
 
+VARIANTS = [(tm, 0, s) for tm in (16, 32, 64, 128) for s in (1, 2, 4, 8)] + [(256, 256, 1), (256, 128, 1), (256, 128, 2), (256, 128, 4)]
+
+
+@pytest.mark.parametrize("tile_m,tile_n,slices", VARIANTS)
+@pytest.mark.parametrize("M,N,K", [(1, 40, 1100), (300, 520, 1400), (777, 900, 1025)])
+def test_every_kernel_form(qlib, dev, monkeypatch, tile_m, tile_n, slices, M, N, K):
+    """Each tile and slice count the library has, whatever it would choose: same product, sums and neighbours kept."""
+    a, sa, b, sb = _operands(qlib, dev, M, N, K, False, False, M + K)
+    ref, mags = _product(a, sa, b, sb)
+    old = torch.randn(M, N, device=dev)
+    monkeypatch.setenv("QGEMM_E8M0_TILE_M", str(tile_m))
+    monkeypatch.setenv("QGEMM_E8M0_TILE_N", str(tile_n))
+    monkeypatch.setenv("QGEMM_E8M0_SLICES", str(slices))
+    qlib.lib().qgemm_reload_env()
+    try:
+        c16 = torch.empty(M, N, dtype=torch.bfloat16, device=dev)
+        qlib.fp8_block_mm_e8m0(a, b, sa, sb, c16)
+        wide = torch.full((M + 1, N + 9), 3.0, device=dev)
+        c = wide[:M, 4:N + 4]
+        c.copy_(old)
+        qlib.fp8_block_mm_e8m0(a, b, sa, sb, c, accumulate=True)
+        rc, st = qlib.device_status()
+    finally:
+        monkeypatch.undo()
+        qlib.lib().qgemm_reload_env()
+    assert rc == 0, st
+    _assert_close(c16, ref, mags, K, torch.bfloat16)
+    _assert_close(c, ref + old.double(), mags + old.abs().double(), K, torch.float32)
+    assert bool((wide[:, :4] == 3).all()) and bool((wide[:, N + 4:] == 3).all()) and bool((wide[M] == 3).all())
+
+
 @pytest.mark.parametrize("M,N,K", [(1, 300, 384), (64, 2048, 1000), (300, 520, 1040), (777, 2048, 4001), (2304, 2176, 384)])
 def test_product_accumulates(qlib, dev, M, N, K):
     a, sa, b, sb = _operands(qlib, dev, M, N, K, False, False, M + N)
