@@ -9,6 +9,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -235,9 +236,9 @@ EnvSettings read_env() {
     const char* ot = std::getenv("QGEMM_ONE_TILE");  // 0: never the one-tile-per-CTA kernel variants
     e.one_tile_off = (ot != nullptr && ot[0] == '0') ? 1 : 0;
     e.kgroup = std::max(0, env_int("QGEMM_KGROUP"));  // 0 = the library's choice, 1 = off, 2 / 4 / 8 = K blocks per load
-    e.e8m0_tile_m = std::max(0, env_int("QGEMM_E8M0_TILE_M"));  // tile rows of the power-of-two block-scaled GEMM
+    e.e8m0_tile_m = std::max(0, env_int("QGEMM_E8M0_TILE_M"));  // forms of the power-of-two block-scaled GEMM to choose among
     e.e8m0_tile_n = std::max(0, env_int("QGEMM_E8M0_TILE_N"));
-    e.e8m0_slices = std::max(0, env_int("QGEMM_E8M0_SLICES"));  // its K slices
+    e.e8m0_slices = std::max(0, env_int("QGEMM_E8M0_SLICES"));
     e.host_bands = std::max(0, env_int("QGEMM_HOST_BANDS"));
     e.host_bands_n = std::max(0, env_int("QGEMM_HOST_BANDS_N"));
     return e;
@@ -934,26 +935,64 @@ int int4_dispatch(int out_dtype, int b_layout, const void* A, size_t lda, const 
                          K, tuning, stream);
 }
 
-// Tile and K slices of the power-of-two block-scaled GEMM.
+// Tile and K slices of the power-of-two block-scaled GEMM: tile_m 16, 32 or 64 tokens by 128 columns with 1, 2, 4 or 8 slices
+// (gemm_e8m0_small_kernel), or CTA pairs on 256 x 128 (1 or 2 slices) or 256 x 256.
 struct E8m0Plan {
     int tile_m, tile_n, slices;
 };
-E8m0Plan plan_e8m0(size_t M, size_t N, int kb_total, int sms) {
-    E8m0Plan pl;
-    pl.tile_m = M <= 16 ? 16 : (M <= 32 ? 32 : (M <= 64 ? 64 : 128));
-    pl.tile_n = 128;
-    const long long tiles = static_cast<long long>((M + pl.tile_m - 1) / pl.tile_m) * static_cast<long long>((N + 127) / 128);
-    pl.slices = 1;
-    while (pl.slices < 8 && tiles * pl.slices * 2 <= 2ll * sms && kb_total >= pl.slices * 2) pl.slices *= 2;
-    if (M > 512 && N > 512) pl = {256, 256, 1};
-    if (g_env.e8m0_tile_m > 0) {
-        pl.tile_m = g_env.e8m0_tile_m;
-        pl.tile_n = pl.tile_m == 256 ? 256 : 128;
-        pl.slices = 1;
+
+// Estimated microseconds, from times measured on B200 (148 SMs, operands not in L2), each figure with sizes it was read from.
+// A launch costs 3 us, and a small tile's results up to 0.6 more; a K block of a small tile 0.20 / 0.21 / 0.265 us (16 / 32
+// / 64 tokens) alone on its SM, 0.28 / 0.30 / 0.34 with another beside it (1 x 4096 x 4096 in 1 to 8 slices, 1024 x 1024 x
+// 8192, 256 x 8192 x 8192), of a 256 x 128 pair tile 0.235 (512 x 4096 x 4096), of a 256 x 256 one 0.345 (2048^3, 512 x
+// 7168 x 7168, 4096^3). Reading alone takes the bytes at 7.1 TB/s once 1.3 CTAs an SM pull (1 x 7168 x 7168: 112 CTAs 12.7
+// us, 224 CTAs 10.9).
+double estimate_e8m0(const E8m0Plan& pl, size_t M, size_t N, size_t K, int sms) {
+    const double kb = static_cast<double>((K + 127) / 128);
+    const double tiles = static_cast<double>((M + pl.tile_m - 1) / pl.tile_m) * static_cast<double>((N + pl.tile_n - 1) / pl.tile_n);
+    const double ctas = tiles * pl.slices * (pl.tile_m == 256 ? 2 : 1);
+    const double bytes = static_cast<double>(M) * K + static_cast<double>(N) * K + 2.0 * M * N;
+    const double hbm = bytes / (7.1e6 * std::min(1.0, 0.5 + 0.5 * ctas / (1.3 * sms)));
+    const double slice_kb = std::ceil(kb / pl.slices);
+    if (pl.tile_m == 256) {
+        if (pl.slices > 1) {  // clusters of four CTAs, one to an SM: not all SMs can be covered
+            const double at_once = std::floor(sms / 4 * 0.9);
+            return 6.0 + std::max(std::ceil(tiles / at_once) * (slice_kb * 0.245 + 2.0) - 2.0, hbm);
+        }
+        const double rounds = std::ceil(tiles / (sms / 2));
+        if (pl.tile_n == 128) return 4.6 + std::max(rounds * (kb * 0.235 + 1.3), hbm);
+        return 6.5 + std::max(rounds * (kb * 0.345 + 1.0), hbm);
     }
-    if (pl.tile_m == 256 && g_env.e8m0_tile_n > 0) pl.tile_n = g_env.e8m0_tile_n;
-    if (g_env.e8m0_slices > 0 && g_env.e8m0_slices <= kb_total) pl.slices = g_env.e8m0_slices;
-    return pl;
+    // clusters of four and eight do not fill every SM's two places
+    const double places = 2.0 * sms * (pl.slices == 8 ? 0.87 : (pl.slices == 4 ? 0.95 : 1.0));
+    const double rounds = std::ceil(ctas / places);
+    const bool shared = ctas > sms;
+    const double per_kb = pl.tile_m == 16 ? (shared ? 0.28 : 0.20) : (pl.tile_m == 32 ? (shared ? 0.30 : 0.21) : (shared ? 0.34 : 0.265));
+    // results; for 16 and 32 tokens also the weights' second reading where there are more tokens
+    const double out = (pl.tile_m == 16 ? 0.0 : (pl.tile_m == 32 ? 0.4 : 0.6)) + (pl.tile_m < 64 && M > static_cast<size_t>(pl.tile_m) ? 0.2 : 0.0);
+    const double join = (pl.slices == 8 ? 1.0 : (pl.slices == 4 ? 0.6 : (pl.slices == 2 ? 0.5 : 0.0))) * (1.0 + pl.tile_m / 32.0);
+    return 3.0 + out + join + 2.0 * (rounds - 1.0) + std::max(rounds * slice_kb * per_kb, hbm);
+}
+
+E8m0Plan plan_e8m0(size_t M, size_t N, size_t K, int sms) {
+    static const E8m0Plan kForms[] = {{16, 128, 1}, {16, 128, 2}, {16, 128, 4}, {16, 128, 8}, {32, 128, 1},
+                                      {32, 128, 2}, {32, 128, 4}, {32, 128, 8}, {64, 128, 1}, {64, 128, 2},
+                                      {64, 128, 4}, {64, 128, 8}, {256, 128, 1}, {256, 128, 2}, {256, 256, 1}};
+    const int kb = static_cast<int>((K + 127) / 128);
+    E8m0Plan best = kForms[0];
+    double best_us = 1e30;
+    for (const E8m0Plan& f : kForms) {
+        if (f.slices > kb) continue;
+        if ((g_env.e8m0_tile_m > 0 && f.tile_m != g_env.e8m0_tile_m) || (g_env.e8m0_tile_n > 0 && f.tile_n != g_env.e8m0_tile_n) ||
+            (g_env.e8m0_slices > 0 && f.slices != g_env.e8m0_slices))
+            continue;
+        const double us = estimate_e8m0(f, M, N, K, sms);
+        if (us < best_us) {
+            best = f;
+            best_us = us;
+        }
+    }
+    return best;
 }
 
 int blockscale_dispatch(int out_dtype, int a_layout, int b_layout, const void* A, size_t lda, const void* B,
@@ -1084,7 +1123,7 @@ int e8m0_dispatch(int out_dtype, const void* A, size_t lda, const uint8_t* a_sca
     p.status = st->status;
     p.c_vec_ok = reinterpret_cast<uintptr_t>(C) % (4 * out_bytes) == 0 && ldc % 4 == 0;
 
-    const E8m0Plan plan = plan_e8m0(M, N, p.kb_total, st->sm_count);
+    const E8m0Plan plan = plan_e8m0(M, N, K, st->sm_count);
     CUtensorMap ta, tb, tc;
     p.m_tiles = static_cast<int>((M + plan.tile_m - 1) / plan.tile_m);
     p.n_tiles = static_cast<int>((N + plan.tile_n - 1) / plan.tile_n);

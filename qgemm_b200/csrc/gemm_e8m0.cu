@@ -66,7 +66,7 @@ cudaError_t launch_pair_one(const CUtensorMap& ta, const CUtensorMap& tb, const 
     constexpr int smem = E8PairSmem<BN>::kDynamicBytes;
     static_assert(smem <= 227 * 1024, "dynamic shared memory of one CTA");
     static bool configured[64] = {};
-    return launch_e8(gemm_e8m0_pair_kernel<OUT, BN>, configured, smem, 2ll * clusters, E8PairSmem<BN>::kThreads, 1, stream, ta, tb, tc, p);
+    return launch_e8(gemm_e8m0_pair_kernel<OUT, BN>, configured, smem, 2ll * clusters, kE8Threads, 1, stream, ta, tb, tc, p);
 }
 
 template <int BN>
@@ -85,7 +85,7 @@ cudaError_t launch_pair_split(const CUtensorMap& ta, const CUtensorMap& tb, cons
     static_assert(E8PairKSmem::kDynamicBytes <= 227 * 1024, "dynamic shared memory of one CTA");
     static bool configured[64] = {};
     return launch_e8(gemm_e8m0_pair_split_kernel<S>, configured, E8PairKSmem::kDynamicBytes,
-                     static_cast<long long>(p.m_tiles) * p.n_tiles * 2 * S, E8PairKSmem::kThreads, 2 * S, stream, ta, tb, p);
+                     static_cast<long long>(p.m_tiles) * p.n_tiles * 2 * S, kE8Threads, 2 * S, stream, ta, tb, p);
 }
 
 }  // namespace
@@ -93,7 +93,6 @@ cudaError_t launch_pair_split(const CUtensorMap& ta, const CUtensorMap& tb, cons
 cudaError_t launch_e8m0_pair(int tile_n, int slices, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc,
                              const E8m0Params& p, int clusters, cudaStream_t stream) {
     if (slices == 2 && tile_n == 128) return launch_pair_split<2>(ta, tb, p, stream);
-    if (slices == 4 && tile_n == 128) return launch_pair_split<4>(ta, tb, p, stream);
     if (slices != 1) return cudaErrorInvalidValue;
     return tile_n == 256 ? launch_pair<256>(ta, tb, tc, p, clusters, stream) : launch_pair<128>(ta, tb, tc, p, clusters, stream);
 }
@@ -104,7 +103,6 @@ cudaError_t launch_e8m0_small(int tokens_per_tile, int slices, const CUtensorMap
         case 16: return launch_small<16>(slices, ta, tb, p, stream);
         case 32: return launch_small<32>(slices, ta, tb, p, stream);
         case 64: return launch_small<64>(slices, ta, tb, p, stream);
-        case 128: return launch_small<128>(slices, ta, tb, p, stream);
         default: return cudaErrorInvalidValue;
     }
 }

@@ -8,13 +8,15 @@
 // which stays in tensor memory for the whole of K, and the product runs at the plain FP8 kernels' pace.
 //
 // The instruction takes one scale per row and 32 elements of K; a 128-wide block is four instructions with the same scale
-// id. One tensor-memory word holds a row's scales of four K blocks (a "chunk"), so a chunk's scales are 512 bytes per 128
-// rows. They come from global memory in the caller's plain layout ([K block][row], or [K block][row / 128]) through a warp
-// that transposes them into words, 16 bytes a lane, and from there with tcgen05.cp.
+// id. One tensor-memory word holds a row's scales of four K blocks (a "chunk"); the 128 rows of an operand take four columns
+// of 32 lanes, repeated over the four lane quadrants. They come from global memory in the caller's plain layout ([K
+// block][row], or [K block][row / 128]) through four warps, one a quadrant: a warp a 128 rows loads words and turns them into
+// a row's four K blocks, and after an exchange through shared memory every warp stores all of them to its quadrant.
+// (Shared memory -> tensor memory with tcgen05.cp takes its place among the MMAs instead: at 4096 x 7168 x 7168 the product
+// took 156 us with it, 139 with the copies left out.)
 //
-// Barriers besides the ring's full / empty and the accumulators': sfull[slot] (a chunk's scales are in shared memory),
-// sempty[slot] (the chunk's last MMA has completed: its shared-memory slot and its tensor-memory columns, same index, are
-// free). All waits are bounded as in gemm_sm100.cuh.
+// Barriers besides the ring's full / empty and the accumulators': sfull[c] (a chunk's scales are in columns c), sdone[c]
+// (the chunk's last MMA has completed: columns c are free). All waits are bounded as in gemm_sm100.cuh.
 #pragma once
 #include "gemm_sm100.cuh"
 
@@ -38,8 +40,8 @@ struct E8m0Params {
     int* status;
 };
 
-constexpr int kE8Slots = 4;  // chunks of scales in flight
-constexpr int kE8Threads = 256;  // producer, MMA issuer, four epilogue warps, two scale warps
+constexpr int kE8Cols = 4;       // chunks of scales in tensor memory
+constexpr int kE8Threads = 320;  // producer, MMA issuer, four epilogue warps, four scale warps (6 .. 9)
 enum : int { ROLE_SCALES = 4 };
 
 // One operand's scales on their way from global to shared memory.
@@ -54,10 +56,9 @@ struct ScaleSource {
 // boundary (any M, any base address). No word is touched that holds none of the operand's scales. A row or K block that
 // does not exist gets some other one's scale: its products are zeros in rows of C that are not stored, or are not made.
 //
-// load_scales uses nothing that it loads, and the warps that fill the slots keep kE8Ahead chunks loading: a chunk must not
-// cost a memory latency each, which under the ring's own traffic is more than the tensor cores take for it (measured at
-// 4096 x 7168 x 7168, row-scaled B: 404 us with one load waited for at a time, 194 with one chunk at a time, 157 with
-// four in flight).
+// load_scales uses nothing that it loads, and a scale warp keeps kE8Ahead chunks loading: a chunk must not cost a memory
+// latency each, which under the ring's own traffic is more than the tensor cores take for it (measured at 4096 x 7168 x
+// 7168, row-scaled B: 404 us with one load waited for at a time, 194 with one chunk at a time, 157 with four in flight).
 constexpr int kE8Ahead = 4;
 struct ScaleWords {
     uint32_t lo[4], hi[4];
@@ -82,7 +83,8 @@ __device__ __forceinline__ void load_scales(ScaleWords& out, const ScaleSource& 
         if (off != 0) out.hi[i] = __ldg(words + min(lane + 1, last));
     }
 }
-// Into the 512 bytes that tc_copy_scales reads: row r's four K blocks as a word at (r % 32) * 16 + (r / 32) * 4.
+// Into 512 bytes of shared memory: row r's four K blocks as a word at (r % 32) * 16 + (r / 32) * 4, so that lane l finds the
+// words of its four columns, rows l, 32 + l, 64 + l and 96 + l, side by side.
 __device__ __forceinline__ void put_scales(uint32_t dst, const ScaleWords& c, const ScaleSource& s, int row0, int kb0, int n,
                                            int lane) {
     if (s.shift != 0) {
@@ -107,45 +109,76 @@ __device__ __forceinline__ void put_scales(uint32_t dst, const ScaleWords& c, co
     }
 }
 
-// The scale warp of a kernel whose CTA has one K range [kb0, kb1) of one tile: `start` loads the first chunks (before the
-// CTA-wide barrier), `run` fills the slots and arrives on sfull (at cluster address full_at(slot)).
+// The four scale warps, over the chunks of K blocks [kb0, kb1) of work items first, first + step, ... < last. Unit u = 0 ..
+// UNITS - 1 is 128 rows of an operand, loaded by scale warp u from row rows(work item). `start` sends the first loads on their
+// way (before the CTA-wide barrier); `run` needs tensor memory, and is executed by all four warps to the end whatever
+// happens, because they meet at a barrier of their own for every chunk: after a wait that ran out they only meet.
+template <int UNITS>
 struct ScaleFeeder {
     ScaleSource src;
-    int row0, kb0, kb1, lane;
+    int g, lane;  // scale warp 0 .. 3
+    int first, last, step, kb0, kb1;
     ScaleWords buf[kE8Ahead];
-    __device__ __forceinline__ void start() {
-#pragma unroll
-        for (int i = 0; i < kE8Ahead; ++i)
-            if (kb0 + 4 * i < kb1) load_scales(buf[i], src, row0, kb0 + 4 * i, min(4, kb1 - kb0 - 4 * i), lane);
+    struct Place {
+        int w, kb, row0;
+    } ahead;
+    template <typename Rows>
+    __device__ __forceinline__ void advance(Place& c, Rows rows) {
+        c.kb += 4;
+        if (c.kb >= kb1) {
+            c.kb = kb0;
+            c.w += step;
+            if (c.w < last) c.row0 = rows(c.w);
+        }
     }
-    // Chunk c goes to slot c % kE8Slots; free(slot, parity) waits for it and says whether to go on.
-    template <typename Free, typename Put>
-    __device__ __forceinline__ bool run(Free free, Put filled, uint32_t slots, uint32_t slot_bytes) {
-        static_assert(kE8Ahead == kE8Slots, "one buffer a slot");
-        uint32_t parity = 1;  // the first pass over the slots finds them free
-        for (int kc = kb0; kc < kb1; kc += 4 * kE8Ahead, parity ^= 1u) {
+    template <typename Rows>
+    __device__ __forceinline__ void fetch(ScaleWords& to, Rows rows) {
+        if (g >= UNITS || ahead.w >= last) return;
+        load_scales(to, src, ahead.row0, ahead.kb, min(4, kb1 - ahead.kb), lane);
+        advance(ahead, rows);
+    }
+    template <typename Rows>
+    __device__ __forceinline__ void start(Rows rows) {
+        ahead = {first, kb0, rows(first)};
+#pragma unroll
+        for (int i = 0; i < kE8Ahead; ++i) fetch(buf[i], rows);
+    }
+    // exchange: 2 * UNITS * 512 bytes of shared memory; tmem: the scale columns (chunk c's at (c % kE8Cols) * 4 * UNITS);
+    // free(column, parity) waits for a column's MMAs, ready(column) arrives on its sfull.
+    template <typename Rows, typename Free, typename Ready>
+    __device__ __forceinline__ void run(Rows rows, uint32_t exchange, uint32_t tmem, int quadrant, Free free, Ready ready) {
+        static_assert(kE8Ahead == kE8Cols && kE8Ahead % 2 == 0, "one buffer a column set, two exchange areas");
+        const uint32_t mine = tmem + (static_cast<uint32_t>(quadrant * 32) << 16);
+        Place put = {first, kb0, rows(first)};
+        uint32_t parity = 1;  // the first pass over the columns finds them free
+        bool ok = true;
+        while (put.w < last) {
 #pragma unroll
             for (int i = 0; i < kE8Ahead; ++i) {
-                const int k = kc + 4 * i;
-                if (k >= kb1) break;
-                if (!free(i, parity, k)) return false;
-                put_scales(slots + i * slot_bytes, buf[i], src, row0, k, min(4, kb1 - k), lane);
-                const int ahead = k + 4 * kE8Ahead;
-                __syncwarp();
-                filled(i);
-                if (ahead < kb1) load_scales(buf[i], src, row0, ahead, min(4, kb1 - ahead), lane);
+                if (put.w >= last) break;
+                const uint32_t area = exchange + (i & 1) * (UNITS * 512);
+                if (g < UNITS) put_scales(area + g * 512, buf[i], src, put.row0, put.kb, min(4, kb1 - put.kb), lane);
+                fetch(buf[i], rows);
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                ok = ok && __all_sync(0xffffffffu, free(i, parity, put.kb));
+                if (ok) {
+                    ptx::tc_fence_after();
+                    uint4 v[UNITS];
+#pragma unroll
+                    for (int u = 0; u < UNITS; ++u) v[u] = ptx::ld_shared_v4(area + u * 512 + lane * 16);
+#pragma unroll
+                    for (int u = 0; u < UNITS; ++u) ptx::tmem_st_32x32b_x4(mine + i * (4 * UNITS) + u * 4, v[u]);
+                    ptx::tmem_st_wait();
+                    ptx::tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) ready(i);
+                }
+                advance(put, rows);
             }
+            parity ^= 1u;
         }
-        return true;
     }
 };
-
-// wait_bounded for a barrier that another CTA of the cluster arrives on after writing its own shared memory.
-__device__ __forceinline__ bool wait_bounded_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status,
-                                                     int role, int where, uint32_t peer_abort) {
-    if (!wait_bounded(bar, parity, abort_flag, status, role, where, peer_abort)) return false;
-    return ptx::mbar_try_wait_cluster(bar, parity);  // complete already: this orders the peer's writes
-}
 
 __device__ __forceinline__ void e8_decode(int w, const E8m0Params& p, int& m_blk, int& n_blk) {
     const int group_sz = p.group_m * p.n_tiles;
@@ -162,7 +195,7 @@ constexpr int kE8RowWords = 128 + 4;  // a row of 128 partial sums in shared mem
 // Adds up the S partial tiles ([rows][kE8RowWords] fp32 at the start of the shared memory of cluster CTAs first, first + STEP,
 // ...) in that order and stores the sums to C[m0 ..][n0 .. n0 + 128]. The `rows` valid rows are dealt out over the S CTAs, of
 // which this is number `part`; a warp takes a row, a lane four columns.
-template <int S, int STEP, int WARPS = kE8Threads / 32>
+template <int S, int STEP>
 __device__ __forceinline__ void sum_and_store(const E8m0Params& p, uint32_t smem_base, uint32_t first, uint32_t part, int m0,
                                               int rows, int n0) {
     const int warp = static_cast<int>(threadIdx.x) >> 5, lane = static_cast<int>(threadIdx.x) & 31;
@@ -172,7 +205,7 @@ __device__ __forceinline__ void sum_and_store(const E8m0Params& p, uint32_t smem
     const int n_valid = min(4, p.N - n);
     if (n_valid <= 0) return;
     const bool vec = p.c_vec_ok != 0 && n_valid == 4;
-    for (int r = static_cast<int>(part) * per + warp; r < r1; r += WARPS) {
+    for (int r = static_cast<int>(part) * per + warp; r < r1; r += kE8Threads / 32) {
         const uint32_t own = smem_base + static_cast<uint32_t>((r * kE8RowWords + lane * 4) * 4);
         float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         uint32_t w[S][4];
@@ -223,7 +256,7 @@ __device__ __forceinline__ void sum_and_store(const E8m0Params& p, uint32_t smem
 
 // ==================================================================================== small and middling M
 // Roles of the operands exchanged: the 128 rows of the instruction are rows of B (output columns), its N = TM columns are
-// rows of A (tokens), 16 to 128 of them, so a few tokens cost a few columns of work instead of a 128-row tile of padding,
+// rows of A (tokens), 16 to 64 of them, so a few tokens cost a few columns of work instead of 128 rows of padding,
 // and a lane of the accumulator is an output column: C's rows leave as contiguous runs.
 //
 // With few tokens the product is one pass over B, bounded by HBM. Every SM has to pull, so K is cut over the S CTAs of a
@@ -236,20 +269,19 @@ struct E8SmallSmem {
     static constexpr int kStages = TM <= 32 ? 5 : 4;
     static constexpr int kTiles = kStages * (kBStage + kAStage);
     static_assert(TM * kE8RowWords * 4 <= kTiles, "the partial tile lies over the ring");
-    static constexpr int kScaleOffset = kTiles;
-    static constexpr int kScaleSlot = 1024;  // 128 rows of B, then up to 128 of A
-    static constexpr int kBarOffset = kScaleOffset + kE8Slots * kScaleSlot;
-    static constexpr int kBars = 2 * kStages + 2 * kE8Slots + 1;
+    static constexpr int kScaleOffset = kTiles;  // exchange areas: 128 rows of B, 128 of A
+    static constexpr int kBarOffset = kScaleOffset + 2 * 2 * 512;
+    static constexpr int kBars = 2 * kStages + 2 * kE8Cols + 1;
     static constexpr int kMiscOffset = kBarOffset + kBars * 8;
     static constexpr int kTotal = kMiscOffset + 16;
     static constexpr int kDynamicBytes = kTotal + 1024;
     static constexpr uint32_t kScaleCol = TM < 32 ? 32 : TM;  // accumulator columns before the scales'
-    static constexpr uint32_t kTmemCols = TM <= 32 ? 64 : (TM == 64 ? 128 : 256);
-    static_assert(kScaleCol + kE8Slots * 8 <= kTmemCols, "tensor-memory columns");
+    static constexpr uint32_t kTmemCols = TM <= 32 ? 64 : 128;
+    static_assert(kScaleCol + kE8Cols * 8 <= kTmemCols, "tensor-memory columns");
 };
 
 template <int TM, int S>
-__global__ void __launch_bounds__(kE8Threads)
+__global__ void __launch_bounds__(kE8Threads, 2)
 gemm_e8m0_small_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                        const E8m0Params p) {
     using L = E8SmallSmem<TM>;
@@ -265,8 +297,8 @@ gemm_e8m0_small_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
     const uint32_t bar_full = smem_base + L::kBarOffset;
     const uint32_t bar_empty = bar_full + STAGES * 8;
     const uint32_t bar_sfull = bar_empty + STAGES * 8;
-    const uint32_t bar_sempty = bar_sfull + kE8Slots * 8;
-    const uint32_t bar_tfull = bar_sempty + kE8Slots * 8;
+    const uint32_t bar_sdone = bar_sfull + kE8Cols * 8;
+    const uint32_t bar_tfull = bar_sdone + kE8Cols * 8;
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + L::kMiscOffset);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMiscOffset + 4);
 
@@ -291,9 +323,9 @@ gemm_e8m0_small_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
             ptx::mbar_init(bar_full + lane * 8, 1);
             ptx::mbar_init(bar_empty + lane * 8, 1);
         }
-        if (lane < kE8Slots) {
-            ptx::mbar_init(bar_sfull + lane * 8, 2);
-            ptx::mbar_init(bar_sempty + lane * 8, 1);
+        if (lane < kE8Cols) {
+            ptx::mbar_init(bar_sfull + lane * 8, 4);  // the scale warps
+            ptx::mbar_init(bar_sdone + lane * 8, 1);
         }
         if (lane == 0) {
             ptx::mbar_init(bar_tfull, 1);
@@ -314,17 +346,20 @@ gemm_e8m0_small_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
         ptx::tmem_alloc(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), L::kTmemCols);
         ptx::tmem_relinquish();
     }
-    // the scale warps (6: B's, 7: A's) send their first loads on their way
+    // the first loads of the scales, B's (unit 0) and A's (unit 1), are on their way too
     const bool of_a = warp == 7;
-    ScaleFeeder feeder;
+    ScaleFeeder<2> feeder;
+    auto scale_rows = [&](int) { return of_a ? m0 : n0; };
     if (warp >= 6) {
         feeder.src = of_a ? ScaleSource{p.a_scale, p.a_rows, p.a_shift, p.M} : ScaleSource{p.b_scale, p.b_rows, p.b_shift, p.N};
-        feeder.row0 = of_a ? m0 : n0;
+        feeder.g = warp - 6;
+        feeder.lane = lane;
+        feeder.first = 0;
+        feeder.last = feeder.step = 1;
         feeder.kb0 = kb0;
         feeder.kb1 = kb1;
-        feeder.lane = lane;
         ptx::pdl_wait();
-        feeder.start();
+        feeder.start(scale_rows);
     }
     ptx::tc_fence_before();
     __syncthreads();
@@ -361,18 +396,14 @@ gemm_e8m0_small_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA issuer
         if (ptx::elect_one()) {
-            uint32_t stage = 0, phase = 0, slot = 0, sphase = 0;
+            uint32_t stage = 0, phase = 0, col = 0, cphase = 0;
             bool ok = true;
             for (int kc = kb0; ok && kc < kb1; kc += 4) {
-                if (!wait_bounded(bar_sfull + slot * 8, sphase, abort_flag, p.status, ROLE_MMA, -1 - kc)) {
+                if (!wait_bounded(bar_sfull + col * 8, cphase, abort_flag, p.status, ROLE_MMA, -1 - kc)) {
                     ok = false;
                     break;
                 }
-                ptx::fence_proxy_async_smem();  // what the scale warps wrote, for the copy
-                ptx::tc_fence_after();
-                const uint32_t sb_tmem = tmem_base + L::kScaleCol + slot * 8, sa_tmem = sb_tmem + 4;
-                ptx::tc_copy_scales(sb_tmem, ptx::make_scale_desc(smem_s + slot * L::kScaleSlot));
-                ptx::tc_copy_scales(sa_tmem, ptx::make_scale_desc(smem_s + slot * L::kScaleSlot + 512));
+                const uint32_t sb_tmem = tmem_base + L::kScaleCol + col * 8, sa_tmem = sb_tmem + 4;
                 const int n = min(4, kb1 - kc);
                 for (int i = 0; i < n; ++i) {
                     if (!wait_bounded(bar_full + stage * 8, phase, abort_flag, p.status, ROLE_MMA, kc + i)) {
@@ -394,10 +425,10 @@ gemm_e8m0_small_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
                     }
                 }
                 if (!ok) break;
-                ptx::tc_commit(bar_sempty + slot * 8);
-                if (++slot == kE8Slots) {
-                    slot = 0;
-                    sphase ^= 1u;
+                ptx::tc_commit(bar_sdone + col * 8);
+                if (++col == kE8Cols) {
+                    col = 0;
+                    cphase ^= 1u;
                 }
             }
             if (ok) ptx::tc_commit(bar_tfull);
@@ -405,13 +436,13 @@ gemm_e8m0_small_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
         }
     } else if (warp >= 6) {
         // ------------------------------------------------------------ scales
-        auto free = [&](int slot, uint32_t parity, int kc) {
-            return wait_bounded(bar_sempty + slot * 8, parity, abort_flag, p.status, ROLE_SCALES, kc);
+        auto free = [&](int col, uint32_t parity, int kb) {
+            const bool ok = wait_bounded(bar_sdone + col * 8, parity, abort_flag, p.status, ROLE_SCALES, kb);
+            if (!ok) raise_peers();
+            return ok;
         };
-        auto filled = [&](int slot) {
-            if (lane == 0) ptx::mbar_arrive(bar_sfull + slot * 8);
-        };
-        if (!feeder.run(free, filled, smem_s + (of_a ? 512 : 0), L::kScaleSlot)) raise_peers();
+        auto ready = [&](int col) { ptx::mbar_arrive(bar_sfull + col * 8); };
+        feeder.run(scale_rows, smem_s, tmem_base + L::kScaleCol, warp & 3, free, ready);
     } else {
         // ------------------------------------------------------------ accumulator -> own shared memory, a token a row
         const int quad = warp & 3;
@@ -470,34 +501,31 @@ gemm_e8m0_small_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
 // the rest of the drain. The first instruction of a tile waits only for a quarter of its predecessor's epilogue.
 //
 // Scales: the leader's instruction multiplies each CTA's 128 rows by that CTA's A scales, and all 256 columns by the B
-// scales, which both CTAs hold in full; the scale warps of either CTA write their own shared memory and arrive on the
-// leader's `sfull`; one tcgen05.cp of the leader copies in both CTAs.
+// scales, which both CTAs hold in full; the scale warps of either CTA arrive on the leader's `sfull`.
 //
 // With 256 x 128 tiles (twice as many, for problems that have too few of the larger) both accumulators fit side by side.
 template <int BN>
 struct E8PairSmem {
-    static constexpr int kScaleWarps = 1 + BN / 128;  // a warp for each 128 rows of scales
-    static constexpr int kThreads = 32 * (7 + kScaleWarps);  // and one that hands their slots over
+    static constexpr int kUnits = 1 + BN / 128;  // 128 rows of scales each: this CTA's of A, all of B
     static constexpr int kStages = BN == 256 ? 6 : 8;
     static constexpr int kAStage = 128 * 128;
     static constexpr int kBStage = (BN / 2) * 128;
     static constexpr int kTiles = kStages * (kAStage + kBStage);
     static constexpr int kOutOffset = kTiles;  // one 4 KB staging box per epilogue warp
     static constexpr int kScaleOffset = kOutOffset + 4 * 4096;
-    static constexpr int kScaleSlot = 512 + (BN / 128) * 512;  // this CTA's 128 rows of A, all rows of B
-    static constexpr int kBarOffset = kScaleOffset + kE8Slots * kScaleSlot;
-    static constexpr int kBars = 2 * kStages + 3 * kE8Slots + 4;  // full, empty, sfull, sempty, sput, tfull[2], tfree[2]
+    static constexpr int kBarOffset = kScaleOffset + 2 * kUnits * 512;
+    static constexpr int kBars = 2 * kStages + 2 * kE8Cols + 4;  // full, empty, sfull, sdone, tfull[2], tfree[2]
     static constexpr int kMiscOffset = kBarOffset + kBars * 8;
     static constexpr int kTotal = kMiscOffset + 16;
     static constexpr int kDynamicBytes = kTotal + 1024;
     static constexpr uint32_t kAccStep = BN == 256 ? 192 : 128;  // first column of the second accumulator
     static constexpr uint32_t kScaleCol = BN == 256 ? 448 : 256;  // first column of the scales
-    static constexpr uint32_t kScaleCols = 4 + BN / 32;  // columns of a chunk: A's, then B's
-    static_assert(kAccStep + BN <= kScaleCol && kScaleCol + kE8Slots * kScaleCols <= 512, "tensor-memory columns");
+    static constexpr uint32_t kScaleCols = 4 * kUnits;  // columns of a chunk: A's, then B's
+    static_assert(kAccStep + BN <= kScaleCol && kScaleCol + kE8Cols * kScaleCols <= 512, "tensor-memory columns");
 };
 
 template <int OUT, int BN>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(E8PairSmem<BN>::kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kE8Threads, 1)
 gemm_e8m0_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                       const __grid_constant__ CUtensorMap tmap_c, const E8m0Params p) {
     using L = E8PairSmem<BN>;
@@ -518,9 +546,8 @@ gemm_e8m0_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
     const uint32_t bar_full = smem_base + L::kBarOffset;
     const uint32_t bar_empty = bar_full + STAGES * 8;
     const uint32_t bar_sfull = bar_empty + STAGES * 8;
-    const uint32_t bar_sempty = bar_sfull + kE8Slots * 8;
-    const uint32_t bar_sput = bar_sempty + kE8Slots * 8;  // this CTA's scale warps have written their part of a slot
-    const uint32_t bar_tfull = bar_sput + kE8Slots * 8;
+    const uint32_t bar_sdone = bar_sfull + kE8Cols * 8;
+    const uint32_t bar_tfull = bar_sdone + kE8Cols * 8;
     // tfree[0] with overlapping accumulators: a tile's share of the common columns is out; else tfree[a]: accumulator a is
     const uint32_t bar_tfree = bar_tfull + 2 * 8;
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + L::kMiscOffset);
@@ -539,10 +566,9 @@ gemm_e8m0_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
             ptx::mbar_init(bar_full + s * 8, 1);
             ptx::mbar_init(bar_empty + s * 8, 1);
         }
-        for (int s = 0; s < kE8Slots; ++s) {
-            ptx::mbar_init(bar_sfull + s * 8, 2);  // both CTAs
-            ptx::mbar_init(bar_sput + s * 8, L::kScaleWarps);
-            ptx::mbar_init(bar_sempty + s * 8, 1);
+        for (int c = 0; c < kE8Cols; ++c) {
+            ptx::mbar_init(bar_sfull + c * 8, 8);  // four scale warps of each CTA
+            ptx::mbar_init(bar_sdone + c * 8, 1);
         }
         ptx::mbar_init(bar_tfull, 1);
         ptx::mbar_init(bar_tfull + 8, 1);
@@ -598,7 +624,7 @@ gemm_e8m0_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA issuer (leader CTA only)
         if (rank == 0 && ptx::elect_one()) {
-            uint32_t stage = 0, phase = 0, slot = 0, sphase = 0;
+            uint32_t stage = 0, phase = 0, col = 0, cphase = 0;
             uint32_t it = 0;
             bool ok = true;
             for (int w = cluster_id; ok && w < total_work; w += n_clusters, ++it) {
@@ -611,17 +637,11 @@ gemm_e8m0_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
                     if (!wait_bounded(bar_tfree + acc * 8, ((it >> 1) & 1u) ^ 1u, abort_flag, p.status, ROLE_MMA, -1, peer_abort)) break;
                 }
                 for (int kc = 0; ok && kc < p.kb_total; kc += 4) {
-                    if (!wait_bounded_cluster(bar_sfull + slot * 8, sphase, abort_flag, p.status, ROLE_MMA, -2 - kc, peer_abort)) {
+                    if (!wait_bounded(bar_sfull + col * 8, cphase, abort_flag, p.status, ROLE_MMA, -2 - kc, peer_abort)) {
                         ok = false;
                         break;
                     }
-                    ptx::tc_fence_after();
-                    const uint32_t sa_tmem = tmem_base + L::kScaleCol + slot * L::kScaleCols, sb_tmem = sa_tmem + 4;
-                    const uint32_t src = smem_s + slot * L::kScaleSlot;
-                    ptx::tc_copy_scales_pair(sa_tmem, ptx::make_scale_desc(src));
-#pragma unroll
-                    for (int h = 0; h < BN / 128; ++h)
-                        ptx::tc_copy_scales_pair(sb_tmem + 4 * h, ptx::make_scale_desc(src + 512 + 512 * h));
+                    const uint32_t sa_tmem = tmem_base + L::kScaleCol + col * L::kScaleCols, sb_tmem = sa_tmem + 4;
                     const int n = min(4, p.kb_total - kc);
                     for (int i = 0; i < n; ++i) {
                         if (!wait_bounded(bar_full + stage * 8, phase, abort_flag, p.status, ROLE_MMA, kc + i, peer_abort)) {
@@ -643,94 +663,38 @@ gemm_e8m0_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
                         }
                     }
                     if (!ok) break;
-                    ptx::tc_commit_pair(bar_sempty + slot * 8, 3);
-                    if (++slot == kE8Slots) {
-                        slot = 0;
-                        sphase ^= 1u;
+                    ptx::tc_commit_pair(bar_sdone + col * 8, 3);
+                    if (++col == kE8Cols) {
+                        col = 0;
+                        cphase ^= 1u;
                     }
                 }
                 if (ok) ptx::tc_commit_pair(bar_tfull + acc * 8, 3);
             }
         }
-    } else if (warp == 6 + L::kScaleWarps) {
-        // ------------------------------------------------------------ scale slots handed to the issuer (both CTAs). The
-        // proxy fence waits for the memory operations of the warp that executes it, so it has a warp without loads
-        if (ptx::elect_one()) {
-            uint32_t slot = 0, phase = 0;
-            const int chunks = (p.kb_total + 3) / 4;
-            bool ok = true;
-            for (int w = cluster_id; ok && w < total_work; w += n_clusters) {
-                for (int c = 0; c < chunks; ++c) {
-                    if (!wait_bounded(bar_sput + slot * 8, phase, abort_flag, p.status, ROLE_SCALES, -1 - c, peer_abort)) {
-                        ok = false;
-                        break;
-                    }
-                    ptx::fence_proxy_async_smem();
-                    ptx::mbar_arrive_cluster(ptx::mapa_shared(bar_sfull + slot * 8, 0));
-                    if (++slot == kE8Slots) {
-                        slot = 0;
-                        phase ^= 1u;
-                    }
-                }
-            }
-        }
     } else if (warp >= 6) {
-        // ------------------------------------------------------------ scales (both CTAs): warp 6 A's, warp 7 B's first 128
-        // rows, warp 8 (BN = 256) B's others; chunk c, counted through all tiles, goes to slot c % 4
+        // ------------------------------------------------------------ scales (both CTAs)
         const bool of_a = warp == 6;
-        const ScaleSource src = of_a ? ScaleSource{p.a_scale, p.a_rows, p.a_shift, p.M}
-                                     : ScaleSource{p.b_scale, p.b_rows, p.b_shift, p.N};
-        const uint32_t slots = smem_s + static_cast<uint32_t>(warp - 6) * 512u;
-        struct Place {
-            int w, kc, row0;
-        };
-        auto tile_row = [&](Place& c) {
-            if (c.w >= total_work) return;
+        ScaleFeeder<L::kUnits> feeder;
+        auto scale_rows = [&](int w) {
             int m_blk, n_blk;
-            e8_decode(c.w, p, m_blk, n_blk);
-            c.row0 = of_a ? (m_blk * 2 + static_cast<int>(rank)) * 128 : n_blk * BN + (warp - 7) * 128;
+            e8_decode(w, p, m_blk, n_blk);
+            return of_a ? (m_blk * 2 + static_cast<int>(rank)) * 128 : n_blk * BN + (warp - 7) * 128;
         };
-        auto advance = [&](Place& c) {
-            c.kc += 4;
-            if (c.kc >= p.kb_total) {
-                c.kc = 0;
-                c.w += n_clusters;
-                tile_row(c);
-            }
+        feeder.src = of_a ? ScaleSource{p.a_scale, p.a_rows, p.a_shift, p.M} : ScaleSource{p.b_scale, p.b_rows, p.b_shift, p.N};
+        feeder.g = warp - 6;
+        feeder.lane = lane;
+        feeder.first = cluster_id;
+        feeder.last = total_work;
+        feeder.step = n_clusters;
+        feeder.kb0 = 0;
+        feeder.kb1 = p.kb_total;
+        feeder.start(scale_rows);
+        auto free = [&](int col, uint32_t parity, int kb) {
+            return wait_bounded(bar_sdone + col * 8, parity, abort_flag, p.status, ROLE_SCALES, kb, peer_abort);
         };
-        Place put = {cluster_id, 0, 0};
-        tile_row(put);
-        Place ahead = put;
-        ScaleWords buf[kE8Ahead];
-        static_assert(kE8Ahead == kE8Slots, "one buffer a slot");
-#pragma unroll
-        for (int i = 0; i < kE8Ahead; ++i) {
-            if (ahead.w < total_work) {
-                load_scales(buf[i], src, ahead.row0, ahead.kc, min(4, p.kb_total - ahead.kc), lane);
-                advance(ahead);
-            }
-        }
-        uint32_t parity = 1;  // the first pass over the slots finds them free
-        bool ok = true;
-        while (ok && put.w < total_work) {
-#pragma unroll
-            for (int i = 0; i < kE8Ahead; ++i) {
-                if (put.w >= total_work) break;
-                if (!wait_bounded(bar_sempty + i * 8, parity, abort_flag, p.status, ROLE_SCALES, put.kc, peer_abort)) {
-                    ok = false;
-                    break;
-                }
-                put_scales(slots + i * L::kScaleSlot, buf[i], src, put.row0, put.kc, min(4, p.kb_total - put.kc), lane);
-                __syncwarp();
-                if (lane == 0) ptx::mbar_arrive(bar_sput + i * 8);
-                advance(put);
-                if (ahead.w < total_work) {
-                    load_scales(buf[i], src, ahead.row0, ahead.kc, min(4, p.kb_total - ahead.kc), lane);
-                    advance(ahead);
-                }
-            }
-            parity ^= 1u;
-        }
+        auto ready = [&](int col) { ptx::mbar_arrive_remote(ptx::mapa_shared(bar_sfull + col * 8, 0)); };
+        feeder.run(scale_rows, smem_s, tmem_base + L::kScaleCol, warp & 3, free, ready);
     } else {
         // ------------------------------------------------------------ epilogue (both CTAs)
         const int quad = warp & 3;
@@ -844,19 +808,17 @@ struct E8PairKSmem {
     static constexpr int kTiles = kStages * (kAStage + kBStage);
     static_assert(128 * kE8RowWords * 4 <= kTiles, "the partial tile lies over the ring");
     static constexpr int kScaleOffset = kTiles;
-    static constexpr int kScaleSlot = 1024;  // this CTA's 128 rows of A, 128 rows of B
-    static constexpr int kBarOffset = kScaleOffset + kE8Slots * kScaleSlot;
-    static constexpr int kBars = 2 * kStages + 3 * kE8Slots + 1;
+    static constexpr int kBarOffset = kScaleOffset + 2 * 2 * 512;
+    static constexpr int kBars = 2 * kStages + 2 * kE8Cols + 1;
     static constexpr int kMiscOffset = kBarOffset + kBars * 8;
     static constexpr int kTotal = kMiscOffset + 16;
     static constexpr int kDynamicBytes = kTotal + 1024;
-    static constexpr int kThreads = kE8Threads + 32;  // and a warp that hands the scale slots over
     static constexpr uint32_t kScaleCol = 128;
     static constexpr uint32_t kTmemCols = 256;
 };
 
 template <int S>
-__global__ void __launch_bounds__(E8PairKSmem::kThreads, 1)
+__global__ void __launch_bounds__(kE8Threads, 1)
 gemm_e8m0_pair_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                             const E8m0Params p) {
     using L = E8PairKSmem;
@@ -872,9 +834,8 @@ gemm_e8m0_pair_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __
     const uint32_t bar_full = smem_base + L::kBarOffset;
     const uint32_t bar_empty = bar_full + STAGES * 8;
     const uint32_t bar_sfull = bar_empty + STAGES * 8;
-    const uint32_t bar_sempty = bar_sfull + kE8Slots * 8;
-    const uint32_t bar_sput = bar_sempty + kE8Slots * 8;
-    const uint32_t bar_tfull = bar_sput + kE8Slots * 8;
+    const uint32_t bar_sdone = bar_sfull + kE8Cols * 8;
+    const uint32_t bar_tfull = bar_sdone + kE8Cols * 8;
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + L::kMiscOffset);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMiscOffset + 4);
 
@@ -895,10 +856,9 @@ gemm_e8m0_pair_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __
             ptx::mbar_init(bar_full + s * 8, 1);
             ptx::mbar_init(bar_empty + s * 8, 1);
         }
-        for (int s = 0; s < kE8Slots; ++s) {
-            ptx::mbar_init(bar_sfull + s * 8, 2);  // both CTAs of the pair
-            ptx::mbar_init(bar_sput + s * 8, 2);   // A's and B's scale warp
-            ptx::mbar_init(bar_sempty + s * 8, 1);
+        for (int c = 0; c < kE8Cols; ++c) {
+            ptx::mbar_init(bar_sfull + c * 8, 8);  // four scale warps of each CTA of the pair
+            ptx::mbar_init(bar_sdone + c * 8, 1);
         }
         ptx::mbar_init(bar_tfull, 1);
         *abort_flag = 0;
@@ -911,15 +871,16 @@ gemm_e8m0_pair_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __
         ptx::tmem_relinquish_pair();
     }
     const bool of_a = warp == 6;
-    ScaleFeeder feeder;
-    if (warp == 6 || warp == 7) {
+    ScaleFeeder<2> feeder;
+    auto scale_rows = [&](int) { return of_a ? m0 : n0; };
+    if (warp >= 6) {
         feeder.src = of_a ? ScaleSource{p.a_scale, p.a_rows, p.a_shift, p.M} : ScaleSource{p.b_scale, p.b_rows, p.b_shift, p.N};
-        feeder.row0 = of_a ? m0 : n0;
+        feeder.g = warp - 6;
+        feeder.lane = lane;
+        feeder.first = 0;
+        feeder.last = feeder.step = 1;
         feeder.kb0 = kb0;
         feeder.kb1 = kb1;
-        feeder.lane = lane;
-        ptx::pdl_wait();
-        feeder.start();
     }
     ptx::tc_fence_before();
     __syncthreads();
@@ -960,17 +921,14 @@ gemm_e8m0_pair_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __
         // ------------------------------------------------------------ MMA issuer (the pair's leader)
         if (rank == 0 && ptx::elect_one()) {
             const uint16_t both = static_cast<uint16_t>(3u << leader);
-            uint32_t stage = 0, phase = 0, slot = 0, sphase = 0;
+            uint32_t stage = 0, phase = 0, col = 0, cphase = 0;
             bool ok = true;
             for (int kc = kb0; ok && kc < kb1; kc += 4) {
-                if (!wait_bounded_cluster(bar_sfull + slot * 8, sphase, abort_flag, p.status, ROLE_MMA, -1 - kc, 0)) {
+                if (!wait_bounded(bar_sfull + col * 8, cphase, abort_flag, p.status, ROLE_MMA, -1 - kc)) {
                     ok = false;
                     break;
                 }
-                ptx::tc_fence_after();
-                const uint32_t sa_tmem = tmem_base + L::kScaleCol + slot * 8, sb_tmem = sa_tmem + 4;
-                ptx::tc_copy_scales_pair(sa_tmem, ptx::make_scale_desc(smem_s + slot * L::kScaleSlot));
-                ptx::tc_copy_scales_pair(sb_tmem, ptx::make_scale_desc(smem_s + slot * L::kScaleSlot + 512));
+                const uint32_t sa_tmem = tmem_base + L::kScaleCol + col * 8, sb_tmem = sa_tmem + 4;
                 const int n = min(4, kb1 - kc);
                 for (int i = 0; i < n; ++i) {
                     if (!wait_bounded(bar_full + stage * 8, phase, abort_flag, p.status, ROLE_MMA, kc + i)) {
@@ -992,41 +950,25 @@ gemm_e8m0_pair_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __
                     }
                 }
                 if (!ok) break;
-                ptx::tc_commit_pair(bar_sempty + slot * 8, both);
-                if (++slot == kE8Slots) {
-                    slot = 0;
-                    sphase ^= 1u;
+                ptx::tc_commit_pair(bar_sdone + col * 8, both);
+                if (++col == kE8Cols) {
+                    col = 0;
+                    cphase ^= 1u;
                 }
             }
             if (ok) ptx::tc_commit_pair(bar_tfull, both);
             else raise_peers();
         }
-    } else if (warp == 8) {
-        // ------------------------------------------------------------ scale slots handed to the issuer (every CTA)
-        if (ptx::elect_one()) {
-            uint32_t slot = 0, phase = 0;
-            for (int kc = kb0; kc < kb1; kc += 4) {
-                if (!wait_bounded(bar_sput + slot * 8, phase, abort_flag, p.status, ROLE_SCALES, -1 - kc)) {
-                    raise_peers();
-                    break;
-                }
-                ptx::fence_proxy_async_smem();
-                ptx::mbar_arrive_cluster(ptx::mapa_shared(bar_sfull + slot * 8, leader));
-                if (++slot == kE8Slots) {
-                    slot = 0;
-                    phase ^= 1u;
-                }
-            }
-        }
     } else if (warp >= 6) {
         // ------------------------------------------------------------ scales (every CTA)
-        auto free = [&](int slot, uint32_t parity, int kc) {
-            return wait_bounded(bar_sempty + slot * 8, parity, abort_flag, p.status, ROLE_SCALES, kc);
+        auto free = [&](int col, uint32_t parity, int kb) {
+            const bool ok = wait_bounded(bar_sdone + col * 8, parity, abort_flag, p.status, ROLE_SCALES, kb);
+            if (!ok) raise_peers();
+            return ok;
         };
-        auto filled = [&](int slot) {
-            if (lane == 0) ptx::mbar_arrive(bar_sput + slot * 8);
-        };
-        if (!feeder.run(free, filled, smem_s + (of_a ? 0 : 512), L::kScaleSlot)) raise_peers();
+        auto ready = [&](int col) { ptx::mbar_arrive_remote(ptx::mapa_shared(bar_sfull + col * 8, leader)); };
+        feeder.start(scale_rows);
+        feeder.run(scale_rows, smem_s, tmem_base + L::kScaleCol, warp & 3, free, ready);
     } else {
         // ------------------------------------------------------------ accumulator -> own shared memory
         const int quad = warp & 3;
@@ -1056,7 +998,7 @@ gemm_e8m0_pair_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __
     __syncthreads();
     ptx::cluster_arrive();
     ptx::cluster_wait();
-    if (*abort_flag == 0 && m0 < p.M) sum_and_store<S, 2, L::kThreads / 32>(p, smem_base, rank, slice, m0, min(128, p.M - m0), n0);
+    if (*abort_flag == 0 && m0 < p.M) sum_and_store<S, 2>(p, smem_base, rank, slice, m0, min(128, p.M - m0), n0);
 
     // ---------------------------------------------------------------- teardown
     ptx::tc_fence_before();
@@ -1073,10 +1015,10 @@ gemm_e8m0_pair_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __
     }
 }
 
-// tokens_per_tile: 16, 32, 64 or 128; slices: 1, 2, 4 or 8, at most kb_total (gemm_e8m0.cu).
+// tokens_per_tile: 16, 32 or 64; slices: 1, 2, 4 or 8, at most kb_total (gemm_e8m0.cu).
 cudaError_t launch_e8m0_small(int tokens_per_tile, int slices, const CUtensorMap& ta, const CUtensorMap& tb,
                               const E8m0Params& p, cudaStream_t stream);
-// tile_n: 256 or 128 (slices == 1: persistent), 128 with slices 2 or 4.
+// tile_n: 256 or 128 (slices == 1: persistent), 128 with slices == 2.
 cudaError_t launch_e8m0_pair(int tile_n, int slices, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc,
                              const E8m0Params& p, int clusters, cudaStream_t stream);
 

@@ -113,6 +113,11 @@ __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t
 __device__ __forceinline__ void st_shared_u32(uint32_t addr, uint32_t v) {
     asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
 __device__ __forceinline__ void tma_store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void tma_store_wait_read() {
@@ -341,37 +346,18 @@ __host__ __device__ constexpr uint32_t make_idesc_e8m0(uint32_t m, uint32_t n) {
 }
 __host__ __device__ constexpr uint32_t idesc_scale_id(uint32_t id) { return (id << 4) | (id << 29); }
 
-// Descriptor of 32 rows x 16 bytes laid end to end (no swizzle: groups of 8 rows 128 bytes apart), the source of
-// tc_copy_scales: row `lane` = the four words (rows lane, 32 + lane, 64 + lane, 96 + lane) of 128 rows' scales.
-__device__ __forceinline__ uint64_t make_scale_desc(uint32_t smem_addr) {
-    uint64_t d = 0;
-    d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
-    d |= static_cast<uint64_t>(128 >> 4) << 32;  // stride byte offset
-    d |= static_cast<uint64_t>(1) << 46;
-    return d;
+// Registers -> tensor memory: this warp's 32 lanes x 4 consecutive 32-bit columns.
+__device__ __forceinline__ void tmem_st_32x32b_x4(uint32_t taddr, const uint4& v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(v.x), "r"(v.y), "r"(v.z),
+                 "r"(v.w)
+                 : "memory");
 }
-// 512 bytes of shared memory to four columns of tensor memory, repeated over the four lane quadrants. Ordered before
-// the MMAs that the same thread issues after it; a tcgen05.commit covers it.
-__device__ __forceinline__ void tc_copy_scales(uint32_t taddr, uint64_t desc) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-}
-// In both CTAs of the pair, each from its own shared memory.
-__device__ __forceinline__ void tc_copy_scales_pair(uint32_t taddr, uint64_t desc) {
-    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-}
-// try_wait that also orders what another CTA of the cluster wrote before its arrival.
-__device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
-        "selp.u32 %0, 1, 0, p;\n"
-        "}\n"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok != 0;
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// Arrive on a barrier of another CTA of the cluster, ordering (as any arrive does by default) this CTA's own accesses only:
+// enough where what was written is this CTA's own memory, read by its own half of a pair's tcgen05 instruction, and the
+// arrival merely tells the thread that issues it. A cluster-scope release instead costs over a microsecond each.
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_bar) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
 // 3-D tiled fp32 add shared -> global: every element of the box is added once to the tensor's, clipped as a store is.
 __device__ __forceinline__ void tma_add_3d(const CUtensorMap* tmap, uint32_t src_smem, int x, int y, int z) {
