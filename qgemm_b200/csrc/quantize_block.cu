@@ -49,12 +49,11 @@ __device__ __forceinline__ float inverse_scale(uint32_t byte) {
     return byte == 255u ? __uint_as_float(0x7fffffffu) : __uint_as_float((254u - byte) << 23);
 }
 
-// Four codes from four scaled values (cvt: two values an instruction, nearest even; NaN gives 0x7f).
-__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
-    return lo | (hi << 16);
+// Two and four codes from scaled values (cvt: two values an instruction, nearest even; NaN gives 0x7f).
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
 }
+__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) { return __byte_perm(pack2(a, b), pack2(c, d), 0x5410); }
 
 // Eight consecutive elements of a row. `maxima` folds their absolute values' bit patterns into m[] (kWords words, as
 // they lie in the source's type), `widen` gives the eight floats, `as_float_bits` the float pattern of one maximum.
@@ -139,18 +138,20 @@ __device__ __forceinline__ uint32_t turned_offset(int c, int piece) {
 }
 
 // The finished column form of a tile, 128 columns x 128 bytes in shared memory, to qt. A half-warp takes one column.
+template <bool WHOLE>
 __device__ __forceinline__ void store_turned(const uint8_t* turned, const QuantBlockParams& p, int row0, int col0) {
-    const int piece = static_cast<int>(threadIdx.x) & 15;
+    const int piece = static_cast<int>(threadIdx.x) & 15, first = static_cast<int>(threadIdx.x) >> 4;
     const int r = row0 + piece * 8;
     const int n = min(8, p.rows - r);
-    if (n <= 0) return;
+    if (!WHOLE && n <= 0) return;
+    uint8_t* dst = p.qt + static_cast<long long>(col0 + first) * p.ld_qt + r;
+    const long long step = (kQbThreads / 16) * p.ld_qt;
 #pragma unroll
-    for (int i = 0; i < kQb / (kQbThreads / 16); ++i) {
-        const int c = i * (kQbThreads / 16) + (static_cast<int>(threadIdx.x) >> 4);
-        if (col0 + c >= p.cols) break;
+    for (int i = 0; i < kQb / (kQbThreads / 16); ++i, dst += step) {
+        const int c = i * (kQbThreads / 16) + first;
+        if (!WHOLE && col0 + c >= p.cols) break;
         const uint2 v = *reinterpret_cast<const uint2*>(turned + turned_offset(c, piece));
-        uint8_t* dst = p.qt + static_cast<long long>(col0 + c) * p.ld_qt + r;
-        if (n == 8 && p.vec_qt) {
+        if (WHOLE || (n == 8 && p.vec_qt)) {
             *reinterpret_cast<uint2*>(dst) = v;
         } else {
             for (int j = 0; j < n; ++j) dst[j] = static_cast<uint8_t>((j < 4 ? v.x >> (8 * j) : v.y >> (8 * (j - 4))) & 0xffu);
@@ -158,64 +159,84 @@ __device__ __forceinline__ void store_turned(const uint8_t* turned, const QuantB
     }
 }
 
-// One thread's 8 x 8 codes of the column form into the shared tile: code[i] holds the codes of columns 0..3 (lo) and 4..7
-// (hi) of row i; eight rows of one column make the eight bytes that are stored together.
-__device__ __forceinline__ void put_turned(uint8_t* turned, int cgroup, int piece, const uint32_t (&lo)[8], const uint32_t (&hi)[8]) {
+// One thread's 8 x 8 codes of the column form into the shared tile: pair[i][k] holds row i's codes of columns 2 k and 2 k + 1
+// in its low half; eight rows of one column make the eight bytes that are stored together.
+__device__ __forceinline__ void put_turned(uint8_t* turned, int cgroup, int piece, const uint32_t (&pair)[8][4]) {
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        const uint32_t(&w)[8] = half ? hi : lo;
-        uint32_t t[4][2];  // a 4 x 4 byte transposition, twice
+    for (int k = 0; k < 4; ++k) {
+        uint32_t even[2], odd[2];
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-            const uint32_t a = __byte_perm(w[4 * g], w[4 * g + 1], 0x5140), b = __byte_perm(w[4 * g + 2], w[4 * g + 3], 0x5140);
-            const uint32_t c = __byte_perm(w[4 * g], w[4 * g + 1], 0x7362), d = __byte_perm(w[4 * g + 2], w[4 * g + 3], 0x7362);
-            t[0][g] = __byte_perm(a, b, 0x5410);
-            t[1][g] = __byte_perm(a, b, 0x7632);
-            t[2][g] = __byte_perm(c, d, 0x5410);
-            t[3][g] = __byte_perm(c, d, 0x7632);
+            const uint32_t a = __byte_perm(pair[4 * g][k], pair[4 * g + 1][k], 0x5140);
+            const uint32_t b = __byte_perm(pair[4 * g + 2][k], pair[4 * g + 3][k], 0x5140);
+            even[g] = __byte_perm(a, b, 0x5410);
+            odd[g] = __byte_perm(a, b, 0x7632);
         }
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            *reinterpret_cast<uint2*>(turned + turned_offset(cgroup * 8 + half * 4 + j, piece)) = make_uint2(t[j][0], t[j][1]);
+        *reinterpret_cast<uint2*>(turned + turned_offset(cgroup * 8 + 2 * k, piece)) = make_uint2(even[0], even[1]);
+        *reinterpret_cast<uint2*>(turned + turned_offset(cgroup * 8 + 2 * k + 1, piece)) = make_uint2(odd[0], odd[1]);
     }
 }
 
+// The maxima of a warp's sixteen rows from each lane's of its eight (rows of its half-warp): a butterfly that halves the
+// rows a lane is responsible for at every step, 8 exchanges instead of 32; lanes 2 j and 2 j + 1 of a half-warp end up with
+// row j.
+template <typename V>
+__device__ __forceinline__ uint32_t row_maximum(const uint32_t (&m)[8], int lane) {
+    uint32_t a[4], b[2];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const bool up = lane & 8;
+        const uint32_t give = up ? m[k] : m[4 + k], keep = up ? m[4 + k] : m[k];
+        a[k] = V::fold(keep, __shfl_xor_sync(0xffffffffu, give, 8));
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const bool up = lane & 4;
+        const uint32_t give = up ? a[k] : a[2 + k], keep = up ? a[2 + k] : a[k];
+        b[k] = V::fold(keep, __shfl_xor_sync(0xffffffffu, give, 4));
+    }
+    const bool up = lane & 2;
+    uint32_t c = V::fold(up ? b[1] : b[0], __shfl_xor_sync(0xffffffffu, up ? b[0] : b[1], 2));
+    return V::fold(c, __shfl_xor_sync(0xffffffffu, c, 1));
+}
+
+template <bool COL, bool SQUARE>
+struct QuantShared {
+    uint8_t turned[COL ? kQb * kQb : 16];
+    uint32_t part[8][COL && !SQUARE ? kQb : 1];  // column (or whole-tile) maxima of each warp's sixteen rows
+    float col_inv[COL && !SQUARE ? kQb : 1];
+};
+
 // A thread's place in the tile: rows 8 * piece .. + 8 with piece = 0..15, columns 8 * cgroup .. + 8 with cgroup = lane & 15;
-// a load instruction of a warp covers two rows of 128 elements.
-template <typename T, bool ROW, bool COL, bool SQUARE>
-__global__ void __launch_bounds__(kQbThreads)
-quantize_block_kernel(const QuantBlockParams p) {
-    ptx::pdl_launch_dependents();
-    ptx::pdl_wait();
+// a load instruction of a warp covers two rows of 128 elements. WHOLE: the tile lies inside the matrix and everything is
+// aligned to whole vectors.
+template <typename T, bool ROW, bool COL, bool SQUARE, bool WHOLE>
+__device__ __forceinline__ void quantize_tile(const QuantBlockParams& p, QuantShared<COL, SQUARE>& sh) {
     using E = typename Elem<T>::type;
     using V = Eight<T>;
-    __shared__ __align__(16) uint8_t turned[COL ? kQb * kQb : 16];
-    __shared__ uint32_t part[8][COL && !SQUARE ? kQb : 1];  // column (or whole-tile) maxima of each warp's sixteen rows
-    __shared__ float col_inv[COL && !SQUARE ? kQb : 1];
-
     const int lane = static_cast<int>(threadIdx.x) & 31, warp = static_cast<int>(threadIdx.x) >> 5;
     const int cgroup = lane & 15, piece = warp * 2 + (lane >> 4);
     const int row0 = static_cast<int>(blockIdx.y) * kQb, col0 = static_cast<int>(blockIdx.x) * kQb;
     const int r0 = row0 + piece * 8, c0 = col0 + cgroup * 8;
     const E* src = static_cast<const E*>(p.in) + static_cast<long long>(r0) * p.ld_in + c0;
-    const int n_cols = min(8, p.cols - c0);
+    const int n_cols = WHOLE ? 8 : min(8, p.cols - c0);
 
     V v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        if (r0 + i < p.rows && n_cols == 8 && p.vec_in) {
-            v[i].load(src + i * p.ld_in);
+    for (int i = 0; i < 8; ++i, src += p.ld_in) {
+        if (WHOLE || (r0 + i < p.rows && n_cols == 8 && p.vec_in)) {
+            v[i].load(src);
         } else {
             v[i].clear();
             if (r0 + i < p.rows) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    if (j < n_cols) v[i].set(j, src + i * p.ld_in + j);
+                    if (j < n_cols) v[i].set(j, src + j);
             }
         }
     }
 
-    float row_inv[8];
+    float row_inv = 1.0f;  // of row (lane >> 1) & 7 of this half-warp
     float tile_inv = 1.0f;
     if constexpr (SQUARE) {
         uint32_t m = 0u;
@@ -225,9 +246,9 @@ quantize_block_kernel(const QuantBlockParams p) {
             for (int k = 0; k < V::kWords; ++k) m = V::fold(m, v[i].mag(k));
         m = V::both_halves(m);
         m = __reduce_max_sync(0xffffffffu, m);
-        if (lane == 0) part[warp][0] = m;
+        if (lane == 0) sh.part[warp][0] = m;
         __syncthreads();
-        m = part[lane & 7][0];
+        m = sh.part[lane & 7][0];
         m = __reduce_max_sync(0xffffffffu, m);
         const uint32_t byte = scale_byte(m);
         tile_inv = inverse_scale(byte);
@@ -237,20 +258,6 @@ quantize_block_kernel(const QuantBlockParams p) {
             if (COL) p.scale_t[blockIdx.y * nb_c + blockIdx.x] = static_cast<uint8_t>(byte);
         }
     } else {
-        if constexpr (ROW) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                uint32_t m = v[i].mag(0);
-#pragma unroll
-                for (int k = 1; k < V::kWords; ++k) m = V::fold(m, v[i].mag(k));
-#pragma unroll
-                for (int o = 8; o > 0; o >>= 1) m = V::fold(m, __shfl_xor_sync(0xffffffffu, m, o));
-                const uint32_t byte = scale_byte(V::both_halves(m));
-                row_inv[i] = inverse_scale(byte);
-                if (cgroup == i && r0 + i < p.rows)
-                    p.scale[static_cast<long long>(blockIdx.x) * p.rows + r0 + i] = static_cast<uint8_t>(byte);
-            }
-        }
         if constexpr (COL) {
 #pragma unroll
             for (int k = 0; k < V::kWords; ++k) {
@@ -260,60 +267,89 @@ quantize_block_kernel(const QuantBlockParams p) {
                 m = V::fold(m, __shfl_xor_sync(0xffffffffu, m, 16));
                 if (lane < 16) {
                     if constexpr (V::kWords == 8) {
-                        part[warp][cgroup * 8 + k] = m;
+                        sh.part[warp][cgroup * 8 + k] = m;
                     } else {
-                        part[warp][cgroup * 8 + 2 * k] = V::float_bits(m, 0);
-                        part[warp][cgroup * 8 + 2 * k + 1] = V::float_bits(m, 1);
+                        sh.part[warp][cgroup * 8 + 2 * k] = V::float_bits(m, 0);
+                        sh.part[warp][cgroup * 8 + 2 * k + 1] = V::float_bits(m, 1);
                     }
                 }
             }
+        }
+        if constexpr (ROW) {
+            uint32_t m[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                m[i] = v[i].mag(0);
+#pragma unroll
+                for (int k = 1; k < V::kWords; ++k) m[i] = V::fold(m[i], v[i].mag(k));
+            }
+            const uint32_t byte = scale_byte(V::both_halves(row_maximum<V>(m, lane)));
+            row_inv = inverse_scale(byte);
+            const int r = r0 + ((lane >> 1) & 7);
+            if ((lane & 1) == 0 && (WHOLE || r < p.rows))
+                p.scale[static_cast<long long>(blockIdx.x) * p.rows + r] = static_cast<uint8_t>(byte);
+        }
+        if constexpr (COL) {
             __syncthreads();
             if (threadIdx.x < kQb) {
                 const int c = static_cast<int>(threadIdx.x);
-                uint32_t m = part[0][c];
+                uint32_t m = sh.part[0][c];
 #pragma unroll
-                for (int w = 1; w < 8; ++w) m = max(m, part[w][c]);
+                for (int w = 1; w < 8; ++w) m = max(m, sh.part[w][c]);
                 const uint32_t byte = scale_byte(m);
-                col_inv[c] = inverse_scale(byte);
-                if (col0 + c < p.cols)
+                sh.col_inv[c] = inverse_scale(byte);
+                if (WHOLE || col0 + c < p.cols)
                     p.scale_t[static_cast<long long>(blockIdx.y) * p.cols + col0 + c] = static_cast<uint8_t>(byte);
             }
-            __syncthreads();
         }
     }
 
     if constexpr (ROW) {
+        uint8_t* dst = p.q + static_cast<long long>(r0) * p.ld_q + c0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (r0 + i < p.rows && n_cols > 0) {
-                const float s = SQUARE ? tile_inv : row_inv[i];
-                const uint2 codes = make_uint2(
-                    pack4(v[i].value(0) * s, v[i].value(1) * s, v[i].value(2) * s, v[i].value(3) * s),
-                    pack4(v[i].value(4) * s, v[i].value(5) * s, v[i].value(6) * s, v[i].value(7) * s));
-                uint8_t* dst = p.q + static_cast<long long>(r0 + i) * p.ld_q + c0;
-                if (n_cols == 8 && p.vec_q) {
-                    *reinterpret_cast<uint2*>(dst) = codes;
-                } else {
-                    for (int j = 0; j < n_cols; ++j)
-                        dst[j] = static_cast<uint8_t>((j < 4 ? codes.x >> (8 * j) : codes.y >> (8 * (j - 4))) & 0xffu);
-                }
+        for (int i = 0; i < 8; ++i, dst += p.ld_q) {
+            const float s = SQUARE ? tile_inv : __shfl_sync(0xffffffffu, row_inv, (lane & 16) + 2 * i);
+            const uint2 codes = make_uint2(
+                pack4(v[i].value(0) * s, v[i].value(1) * s, v[i].value(2) * s, v[i].value(3) * s),
+                pack4(v[i].value(4) * s, v[i].value(5) * s, v[i].value(6) * s, v[i].value(7) * s));
+            if (WHOLE || (r0 + i < p.rows && n_cols == 8 && p.vec_q)) {
+                *reinterpret_cast<uint2*>(dst) = codes;
+            } else if (r0 + i < p.rows) {
+                for (int j = 0; j < n_cols; ++j)
+                    dst[j] = static_cast<uint8_t>((j < 4 ? codes.x >> (8 * j) : codes.y >> (8 * (j - 4))) & 0xffu);
             }
         }
     }
     if constexpr (COL) {
+        if (!SQUARE) __syncthreads();
         float s[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s[j] = SQUARE ? tile_inv : col_inv[cgroup * 8 + j];
-        uint32_t lo[8], hi[8];
+        for (int j = 0; j < 8; ++j) s[j] = SQUARE ? tile_inv : sh.col_inv[cgroup * 8 + j];
+        uint32_t pair[8][4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            lo[i] = pack4(v[i].value(0) * s[0], v[i].value(1) * s[1], v[i].value(2) * s[2], v[i].value(3) * s[3]);
-            hi[i] = pack4(v[i].value(4) * s[4], v[i].value(5) * s[5], v[i].value(6) * s[6], v[i].value(7) * s[7]);
-        }
-        put_turned(turned, cgroup, piece, lo, hi);
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) pair[i][k] = pack2(v[i].value(2 * k) * s[2 * k], v[i].value(2 * k + 1) * s[2 * k + 1]);
+        put_turned(sh.turned, cgroup, piece, pair);
         __syncthreads();
-        store_turned(turned, p, row0, col0);
+        store_turned<WHOLE>(sh.turned, p, row0, col0);
     }
+}
+
+__device__ __forceinline__ bool whole_tile(const QuantBlockParams& p) {
+    return p.vec_in && p.vec_q && p.vec_qt && static_cast<int>(blockIdx.y + 1) * kQb <= p.rows &&
+           static_cast<int>(blockIdx.x + 1) * kQb <= p.cols;
+}
+
+// Both forms of a 16-bit matrix would take 100 registers, two tiles an SM: held to three (4096 x 7168 25.9 -> 22.3 us).
+template <typename T, bool ROW, bool COL, bool SQUARE>
+__global__ void __launch_bounds__(kQbThreads, ROW && COL && !SQUARE && sizeof(typename Elem<T>::type) == 2 ? 3 : 1)
+quantize_block_kernel(const QuantBlockParams p) {
+    ptx::pdl_launch_dependents();
+    ptx::pdl_wait();
+    __shared__ __align__(16) QuantShared<COL, SQUARE> sh;
+    if (whole_tile(p)) quantize_tile<T, ROW, COL, SQUARE, true>(p, sh);
+    else quantize_tile<T, ROW, COL, SQUARE, false>(p, sh);
 }
 
 // ------------------------------------------------------------------------------------------------ from 8 bits
@@ -337,46 +373,70 @@ __device__ __forceinline__ uint32_t scale_byte_shifted(uint32_t b) {  // from th
     return (b + 0x1fffffu) >> 23;
 }
 
-// Row form -> column form: the 128 x 1 blocks of the values quantised anew. One byte read and one written an element.
-__global__ void __launch_bounds__(kQbThreads)
-requantize_block_kernel(const QuantBlockParams p) {
-    ptx::pdl_launch_dependents();
-    ptx::pdl_wait();
-    __shared__ __align__(16) uint8_t turned[kQb * kQb];
-    __shared__ uint32_t part[8][kQb];
-    __shared__ float col_inv[kQb];
+// Row form -> column form: the 128 x 1 blocks of the values quantised anew. One byte read and one written an element, so
+// what bounds it besides HBM is the arithmetic, and that is done two elements at a time in fp16 wherever fp16 is exact:
+//   u = code * 2^(E_row - S), S the largest of the tile's 128 row scales, is a whole multiple of 2^-24 with 4 significant
+//   bits when all rows are within 2^15 of S, so it is exact (as a subnormal, too), and so are the columns' maxima;
+//   y = u * 2^(S - E_col) has a factor that fp16 holds when the column's maximum is at least 2^-6 (or 0); it is exact, or
+//   below 2^-14 and a zero among the codes however it is rounded.
+// A tile that is not like that (rows far apart, a column of nothing but tiny codes, a NaN) takes the fp32 form below: a
+// tile's choice is the same for all its threads. (All in fp32: 77 us at 16384 x 7168, 15 instructions an element.)
+struct RequantShared {
+    uint8_t turned[kQb * kQb];
+    uint32_t part[8][kQb];
+    uint32_t factor[kQb];
+};
 
-    const int lane = static_cast<int>(threadIdx.x) & 31, warp = static_cast<int>(threadIdx.x) >> 5;
-    const int cgroup = lane & 15, piece = warp * 2 + (lane >> 4);
-    const int row0 = static_cast<int>(blockIdx.y) * kQb, col0 = static_cast<int>(blockIdx.x) * kQb;
-    const int r0 = row0 + piece * 8, c0 = col0 + cgroup * 8;
-    const uint8_t* src = static_cast<const uint8_t*>(p.in) + static_cast<long long>(r0) * p.ld_in + c0;
-    const int n_cols = min(8, p.cols - c0);
-
-    uint2 v[8];
-    uint32_t byte[8];
+// Maxima of eight warps' parts -> the columns' scale bytes, stored; `factor` keeps what multiplies a column's values.
+template <bool WHOLE, typename Byte, typename Factor>
+__device__ __forceinline__ void column_scales(RequantShared& sh, const QuantBlockParams& p, int col0, Byte byte_of, Factor factor_of) {
+    if (threadIdx.x < kQb) {
+        const int c = static_cast<int>(threadIdx.x);
+        uint32_t b = sh.part[0][c];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        v[i] = make_uint2(0u, 0u);
-        byte[i] = 127u;
-        if (r0 + i < p.rows && n_cols > 0) {
-            byte[i] = __ldg(p.in_scale + static_cast<long long>(blockIdx.x) * p.rows + r0 + i);
-            if (n_cols == 8 && p.vec_in) {
-                v[i] = __ldg(reinterpret_cast<const uint2*>(src + i * p.ld_in));
-            } else {
+        for (int w = 1; w < 8; ++w) b = max(b, sh.part[w][c]);
+        const uint32_t e = byte_of(b);
+        sh.factor[c] = factor_of(e);
+        if (WHOLE || col0 + c < p.cols) p.scale_t[static_cast<long long>(blockIdx.y) * p.cols + col0 + c] = static_cast<uint8_t>(e);
+    }
+}
+
+// A thread's codes of the tile; zeros where there is no row or column.
+template <bool WHOLE>
+__device__ __forceinline__ void load_codes(const QuantBlockParams& p, int r0, int c0, uint2 (&v)[8]) {
+    const uint8_t* src = static_cast<const uint8_t*>(p.in) + static_cast<long long>(r0) * p.ld_in + c0;
+    const int n_cols = WHOLE ? 8 : min(8, p.cols - c0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i, src += p.ld_in) {
+        if (WHOLE || (r0 + i < p.rows && n_cols == 8 && p.vec_in)) {
+            v[i] = __ldg(reinterpret_cast<const uint2*>(src));
+        } else {
+            v[i] = make_uint2(0u, 0u);
+            if (r0 + i < p.rows) {
                 for (int j = 0; j < n_cols; ++j) {
-                    const uint32_t c = __ldg(src + i * p.ld_in + j);
+                    const uint32_t c = __ldg(src + j);
                     if (j < 4) v[i].x |= c << (8 * j);
                     else v[i].y |= c << (8 * (j - 4));
                 }
             }
         }
     }
+}
+
+// The fp32 form, for any codes and scales.
+template <bool WHOLE>
+__device__ __noinline__ void requantize_tile_fp32(const QuantBlockParams& p, RequantShared& sh) {
+    const int lane = static_cast<int>(threadIdx.x) & 31, warp = static_cast<int>(threadIdx.x) >> 5;
+    const int cgroup = lane & 15, piece = warp * 2 + (lane >> 4);
+    const int row0 = static_cast<int>(blockIdx.y) * kQb, col0 = static_cast<int>(blockIdx.x) * kQb;
+    uint2 v[8];
+    load_codes<WHOLE>(p, row0 + piece * 8, col0 + cgroup * 8, v);
+    const uint8_t* scales = p.in_scale + static_cast<long long>(blockIdx.x) * p.rows + row0 + piece * 8;
     float s[8];
     uint32_t m[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        s[i] = shifted_scale(byte[i]);
+        s[i] = shifted_scale(WHOLE || row0 + piece * 8 + i < p.rows ? __ldg(scales + i) : 127u);
         float x[4];
         decode4(v[i].x, x);
 #pragma unroll
@@ -388,30 +448,23 @@ requantize_block_kernel(const QuantBlockParams p) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         m[j] = max(m[j], __shfl_xor_sync(0xffffffffu, m[j], 16));
-        if (lane < 16) part[warp][cgroup * 8 + j] = m[j];
+        if (lane < 16) sh.part[warp][cgroup * 8 + j] = m[j];
     }
     __syncthreads();
-    if (threadIdx.x < kQb) {
-        const int c = static_cast<int>(threadIdx.x);
-        uint32_t b = part[0][c];
-#pragma unroll
-        for (int w = 1; w < 8; ++w) b = max(b, part[w][c]);
-        const uint32_t e = scale_byte_shifted(b);
-        // 2^(8 - E) as a float; below E = -119 it does not exist: those columns carry 2^127 and the missing factor is
-        // applied to the values first, marked by the sign
-        col_inv[c] = e == 255u ? __uint_as_float(0x7fffffffu)
-                               : (e >= 8u ? __uint_as_float((262u - e) << 23) : -__uint_as_float((254u - e) << 23));
-        if (col0 + c < p.cols) p.scale_t[static_cast<long long>(blockIdx.y) * p.cols + col0 + c] = static_cast<uint8_t>(e);
-    }
+    // 2^(8 - E) as a float; below E = -119 it does not exist: those columns carry 2^(-E - 1) with the sign set, and 2^9
+    // is applied to the values first
+    column_scales<WHOLE>(
+        sh, p, col0, [](uint32_t b) { return scale_byte_shifted(b); },
+        [](uint32_t e) { return e == 255u ? 0x7fffffffu : (e >= 8u ? (262u - e) << 23 : 0x80000000u | ((253u - e) << 23)); });
     __syncthreads();
     float t[8];
     bool small = false;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        t[j] = col_inv[cgroup * 8 + j];
+        t[j] = __uint_as_float(sh.factor[cgroup * 8 + j]);
         small = small || t[j] < 0.0f;
     }
-    uint32_t lo[8], hi[8];
+    uint32_t pair[8][4];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         float x[4], y[4];
@@ -425,8 +478,8 @@ requantize_block_kernel(const QuantBlockParams p) {
         if (small) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                x[j] = t[j] < 0.0f ? x[j] * 256.0f * -t[j] : x[j] * t[j];
-                y[j] = t[4 + j] < 0.0f ? y[j] * 256.0f * -t[4 + j] : y[j] * t[4 + j];
+                x[j] = t[j] < 0.0f ? x[j] * 512.0f * -t[j] : x[j] * t[j];
+                y[j] = t[4 + j] < 0.0f ? y[j] * 512.0f * -t[4 + j] : y[j] * t[4 + j];
             }
         } else {
 #pragma unroll
@@ -435,80 +488,209 @@ requantize_block_kernel(const QuantBlockParams p) {
                 y[j] *= t[4 + j];
             }
         }
-        lo[i] = pack4(x[0], x[1], x[2], x[3]);
-        hi[i] = pack4(y[0], y[1], y[2], y[3]);
+        pair[i][0] = pack2(x[0], x[1]);
+        pair[i][1] = pack2(x[2], x[3]);
+        pair[i][2] = pack2(y[0], y[1]);
+        pair[i][3] = pack2(y[2], y[3]);
     }
-    put_turned(turned, cgroup, piece, lo, hi);
+    put_turned(sh.turned, cgroup, piece, pair);
     __syncthreads();
-    store_turned(turned, p, row0, col0);
+    store_turned<WHOLE>(sh.turned, p, row0, col0);
+}
+
+__device__ __forceinline__ __half2 half2_of(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
+__device__ __forceinline__ uint32_t bits_of(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+__device__ __forceinline__ __half2 decode2(uint32_t codes) {
+    return __half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(codes & 0xffffu), __NV_E4M3));
+}
+__device__ __forceinline__ uint32_t encode2(__half2 y) { return __nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(y), __NV_SATFINITE, __NV_E4M3); }
+
+template <bool WHOLE>
+__device__ __forceinline__ void requantize_tile(const QuantBlockParams& p, RequantShared& sh) {
+    const int lane = static_cast<int>(threadIdx.x) & 31, warp = static_cast<int>(threadIdx.x) >> 5;
+    const int cgroup = lane & 15, piece = warp * 2 + (lane >> 4);
+    const int row0 = static_cast<int>(blockIdx.y) * kQb, col0 = static_cast<int>(blockIdx.x) * kQb;
+    uint2 v[8];
+    load_codes<WHOLE>(p, row0 + piece * 8, col0 + cgroup * 8, v);
+    // this lane's row's scale, and the largest and smallest of the tile's, in every warp
+    const uint8_t* scales = p.in_scale + static_cast<long long>(blockIdx.x) * p.rows + row0;
+    const int own = piece * 8 + (cgroup >> 1);
+    const bool exists = WHOLE || row0 + own < p.rows;
+    const uint32_t byte = exists ? __ldg(scales + own) : 0u;
+    uint32_t top = 0u, low = 255u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int r = 32 * j + lane;
+        if (WHOLE || row0 + r < p.rows) {
+            const uint32_t b = __ldg(scales + r);
+            top = max(top, b);
+            low = min(low, b);
+        }
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    low = __reduce_min_sync(0xffffffffu, low);
+    if (top == 255u || top - low > 15u) {
+        requantize_tile_fp32<WHOLE>(p, sh);
+        return;
+    }
+    // 2^(E_row - S) in both halves: normal down to 2^-14, 2^-15 a subnormal; the codes of rows that do not exist are zeros
+    const uint32_t below = top - byte;
+    const uint32_t factor_bits = (!exists || below == 15u ? 0x200u : (15u - below) << 10) * 0x10001u;
+    // The codes stay as they are and are decoded twice: that takes half the registers, so five tiles fit on an SM.
+    __half2 f[8], m[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) m[k] = half2_of(0u);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        f[i] = half2_of(__shfl_sync(0xffffffffu, factor_bits, (lane & 16) + 2 * i));
+        m[0] = __hmax2_nan(m[0], __habs2(__hmul2(decode2(v[i].x), f[i])));
+        m[1] = __hmax2_nan(m[1], __habs2(__hmul2(decode2(v[i].x >> 16), f[i])));
+        m[2] = __hmax2_nan(m[2], __habs2(__hmul2(decode2(v[i].y), f[i])));
+        m[3] = __hmax2_nan(m[3], __habs2(__hmul2(decode2(v[i].y >> 16), f[i])));
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        m[k] = __hmax2_nan(m[k], half2_of(__shfl_xor_sync(0xffffffffu, bits_of(m[k]), 16)));
+        if (lane < 16) {
+            sh.part[warp][cgroup * 8 + 2 * k] = bits_of(m[k]) & 0xffffu;
+            sh.part[warp][cgroup * 8 + 2 * k + 1] = bits_of(m[k]) >> 16;
+        }
+    }
+    __syncthreads();
+    bool other = false;
+    if (threadIdx.x < kQb) {
+        const int c = static_cast<int>(threadIdx.x);
+        uint32_t b = sh.part[0][c];
+#pragma unroll
+        for (int w = 1; w < 8; ++w) b = max(b, sh.part[w][c]);
+        // a column's maximum lies in [2^-6, 448] or is 0, or the tile takes the other form (a NaN's pattern lies above)
+        other = b != 0u && (b < 0x2400u || b > 0x5f00u);
+        // E_col - S = exponent - 8, one more when the mantissa is above 1.75, -14 .. 0 here; E_col is at least -127
+        uint32_t e = 127u, factor = 0u;
+        if (b != 0u && !other) {
+            const int d = static_cast<int>((b + 0xffu) >> 10) - 15 - 8;
+            const int byte_of_column = max(0, static_cast<int>(top) + d);
+            e = static_cast<uint32_t>(byte_of_column);
+            factor = static_cast<uint32_t>(15 - (byte_of_column - static_cast<int>(top))) << 10;
+        }
+        sh.factor[c] = factor;
+        if (!other && (WHOLE || col0 + c < p.cols))
+            p.scale_t[static_cast<long long>(blockIdx.y) * p.cols + col0 + c] = static_cast<uint8_t>(e);
+    }
+    if (__syncthreads_or(other)) {
+        requantize_tile_fp32<WHOLE>(p, sh);
+        return;
+    }
+    __half2 t[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) t[k] = half2_of(sh.factor[cgroup * 8 + 2 * k] | (sh.factor[cgroup * 8 + 2 * k + 1] << 16));
+    uint32_t pair[8][4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        pair[i][0] = encode2(__hmul2(__hmul2(decode2(v[i].x), f[i]), t[0]));
+        pair[i][1] = encode2(__hmul2(__hmul2(decode2(v[i].x >> 16), f[i]), t[1]));
+        pair[i][2] = encode2(__hmul2(__hmul2(decode2(v[i].y), f[i]), t[2]));
+        pair[i][3] = encode2(__hmul2(__hmul2(decode2(v[i].y >> 16), f[i]), t[3]));
+    }
+    put_turned(sh.turned, cgroup, piece, pair);
+    __syncthreads();
+    store_turned<WHOLE>(sh.turned, p, row0, col0);
+}
+
+__global__ void __launch_bounds__(kQbThreads, 5)
+requantize_block_kernel(const QuantBlockParams p) {
+    ptx::pdl_launch_dependents();
+    ptx::pdl_wait();
+    __shared__ __align__(16) RequantShared sh;
+    if (whole_tile(p)) requantize_tile<true>(p, sh);
+    else requantize_tile<false>(p, sh);
 }
 
 // out = round(code * 2^E). The product is exact in fp32 (or overflows to an infinity, as the rounded value does), so the
-// conversion to the output type is the one rounding. Eight elements a thread and step.
+// conversion to the output type is the one rounding. A thread has W neighbouring columns (16 bytes of output) of four rows
+// at a time (eight took more registers: 16384 x 7168 to bf16 75 us instead of 59): their loads are all in flight together, a warp's stores cover whole lines, and rows and columns come without a
+// division.
+constexpr int kDequantRows = 4;
 template <int OUT>
-__global__ void __launch_bounds__(kQbThreads)
+__global__ void __launch_bounds__(kQbThreads, 4)
 dequantize_block_kernel(const uint8_t* __restrict__ q, long long ld_q, const uint8_t* __restrict__ scale, int block_shift,
                         long long scale_rows, int rows, int cols, uint8_t* __restrict__ out, long long ld_out, int vec_in,
                         int vec_out) {
     ptx::pdl_launch_dependents();
     ptx::pdl_wait();
     constexpr int OB = OUT == OUT_F32 ? 4 : 2;
-    const int groups = (cols + 7) / 8;
-    const long long total = static_cast<long long>(groups) * rows;
-    const long long step = static_cast<long long>(gridDim.x) * kQbThreads;
-    for (long long g = static_cast<long long>(blockIdx.x) * kQbThreads + threadIdx.x; g < total; g += step) {
-        const long long r = g / groups;
-        const int c = static_cast<int>(g - r * groups) * 8;
-        const int n = min(8, cols - c);
-        const uint8_t* src = q + r * ld_q + c;
-        uint2 v = make_uint2(0u, 0u);
-        if (n == 8 && vec_in) {
-            v = __ldg(reinterpret_cast<const uint2*>(src));
-        } else {
-            for (int j = 0; j < n; ++j) {
-                const uint32_t b = __ldg(src + j);
-                if (j < 4) v.x |= b << (8 * j);
-                else v.y |= b << (8 * (j - 4));
-            }
-        }
-        const uint32_t byte = __ldg(scale + static_cast<long long>(c >> 7) * scale_rows + (r >> block_shift));
-        const float s = byte == 255u ? __uint_as_float(0x7fffffffu)
-                                     : (byte == 0u ? __uint_as_float(0x400000u) : __uint_as_float(byte << 23));
-        float x[8];
-        decode4(v.x, *reinterpret_cast<float(*)[4]>(&x[0]));
-        decode4(v.y, *reinterpret_cast<float(*)[4]>(&x[4]));
+    constexpr int W = 16 / OB, U = kDequantRows;
+    const int c = (static_cast<int>(blockIdx.x) * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x)) * W;
+    if (c >= cols) return;
+    const int n = min(W, cols - c);
+    const uint8_t* scales = scale + static_cast<long long>(c >> 7) * scale_rows;
+    const long long step = static_cast<long long>(gridDim.y) * blockDim.y * U;
+    for (long long r0 = (static_cast<long long>(blockIdx.y) * blockDim.y + threadIdx.y) * U; r0 < rows; r0 += step) {
+        const int nr = static_cast<int>(min(static_cast<long long>(U), rows - r0));
+        const uint8_t* src = q + r0 * ld_q + c;
+        uint32_t v[U][W / 4], byte[U];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] *= s;
-        uint8_t* dst = out + (r * ld_out + c) * OB;
-        if constexpr (OUT == OUT_F32) {
-            if (n == 8 && vec_out) {
-                reinterpret_cast<float4*>(dst)[0] = make_float4(x[0], x[1], x[2], x[3]);
-                reinterpret_cast<float4*>(dst)[1] = make_float4(x[4], x[5], x[6], x[7]);
-            } else {
+        for (int i = 0; i < U; ++i) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (j < n) reinterpret_cast<float*>(dst)[j] = x[j];
-            }
-        } else {
-            uint32_t u[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if constexpr (OUT == OUT_BF16) {
-                    const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
-                    u[j] = *reinterpret_cast<const uint32_t*>(&h);
+            for (int k = 0; k < W / 4; ++k) v[i][k] = 0u;
+            byte[i] = 127u;
+            if (i < nr) {
+                byte[i] = __ldg(scales + ((r0 + i) >> block_shift));
+                if (n == W && vec_in) {
+                    if constexpr (W == 8) {
+                        const uint2 w = __ldg(reinterpret_cast<const uint2*>(src + i * ld_q));
+                        v[i][0] = w.x;
+                        v[i][1] = w.y;
+                    } else {
+                        v[i][0] = __ldg(reinterpret_cast<const uint32_t*>(src + i * ld_q));
+                    }
                 } else {
-                    const __half2 h = __floats2half2_rn(x[2 * j], x[2 * j + 1]);
-                    u[j] = *reinterpret_cast<const uint32_t*>(&h);
+#pragma unroll
+                    for (int j = 0; j < W; ++j)
+                        if (j < n) v[i][j >> 2] |= static_cast<uint32_t>(__ldg(src + i * ld_q + j)) << (8 * (j & 3));
                 }
             }
-            if (n == 8 && vec_out) {
-                *reinterpret_cast<uint4*>(dst) = make_uint4(u[0], u[1], u[2], u[3]);
-            } else {
+        }
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (j < n)
-                        reinterpret_cast<uint16_t*>(dst)[j] =
-                            static_cast<uint16_t>((j & 1) ? (u[j >> 1] >> 16) : (u[j >> 1] & 0xffffu));
+        for (int i = 0; i < U; ++i) {
+            if (i >= nr) break;
+            const float s = byte[i] == 255u ? __uint_as_float(0x7fffffffu)
+                                            : (byte[i] == 0u ? __uint_as_float(0x400000u) : __uint_as_float(byte[i] << 23));
+            float x[W];
+#pragma unroll
+            for (int k = 0; k < W / 4; ++k) decode4(v[i][k], *reinterpret_cast<float(*)[4]>(&x[4 * k]));
+#pragma unroll
+            for (int j = 0; j < W; ++j) x[j] *= s;
+            uint8_t* dst = out + ((r0 + i) * ld_out + c) * OB;
+            if constexpr (OUT == OUT_F32) {
+                if (n == W && vec_out) {
+                    *reinterpret_cast<float4*>(dst) = make_float4(x[0], x[1], x[2], x[3]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < W; ++j)
+                        if (j < n) reinterpret_cast<float*>(dst)[j] = x[j];
+                }
+            } else {
+                uint32_t u[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if constexpr (OUT == OUT_BF16) {
+                        const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
+                        u[j] = *reinterpret_cast<const uint32_t*>(&h);
+                    } else {
+                        const __half2 h = __floats2half2_rn(x[2 * j], x[2 * j + 1]);
+                        u[j] = *reinterpret_cast<const uint32_t*>(&h);
+                    }
+                }
+                if (n == W && vec_out) {
+                    *reinterpret_cast<uint4*>(dst) = make_uint4(u[0], u[1], u[2], u[3]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < W; ++j)
+                        if (j < n)
+                            reinterpret_cast<uint16_t*>(dst)[j] =
+                                static_cast<uint16_t>((j & 1) ? (u[j >> 1] >> 16) : (u[j >> 1] & 0xffffu));
+                }
             }
         }
     }
@@ -559,8 +741,8 @@ int quantize_block_launch(int in_dtype, const void* in, size_t ld_in, size_t row
     p.rows = static_cast<int>(rows);
     p.cols = static_cast<int>(cols);
     p.vec_in = aligned(in, ld_in * es, 16);
-    p.vec_q = aligned(q, ld_q, 8);
-    p.vec_qt = aligned(qt, ld_qt, 8);
+    p.vec_q = q == nullptr || aligned(q, ld_q, 8);
+    p.vec_qt = qt == nullptr || aligned(qt, ld_qt, 8);
     const dim3 grid(static_cast<unsigned>((cols + kQb - 1) / kQb), static_cast<unsigned>((rows + kQb - 1) / kQb));
     cudaError_t e;
     switch (in_dtype) {
@@ -587,6 +769,7 @@ int requantize_block_launch(const void* q, size_t ld_q, const uint8_t* scale, si
     p.rows = static_cast<int>(rows);
     p.cols = static_cast<int>(cols);
     p.vec_in = aligned(q, ld_q, 8);
+    p.vec_q = 1;
     p.vec_qt = aligned(qt, ld_qt, 8);
     const dim3 grid(static_cast<unsigned>((cols + kQb - 1) / kQb), static_cast<unsigned>((rows + kQb - 1) / kQb));
     return launch_pdl(requantize_block_kernel, grid, dim3(kQbThreads), 0, stream, p) == cudaSuccess ? QGEMM_OK : QGEMM_ERR_CUDA;
@@ -602,17 +785,19 @@ int dequantize_block_launch(int out_dtype, const void* q, size_t ld_q, const uin
     if (rows > kMaxSide || cols > kMaxSide) return QGEMM_ERR_INVALID_ARG;
     const size_t es = out_dtype == QGEMM_DTYPE_FP32 ? 4 : 2;
     if (reinterpret_cast<uintptr_t>(out) % es != 0) return QGEMM_ERR_ALIGNMENT;
-    int dev = 0, sms = 148;
-    if (cudaGetDevice(&dev) != cudaSuccess) return QGEMM_ERR_CUDA;
-    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return QGEMM_ERR_CUDA;
-    const size_t groups = ((cols + 7) / 8) * rows;
-    const size_t want = (groups + kQbThreads - 1) / kQbThreads;
-    const unsigned blocks = static_cast<unsigned>(want < static_cast<size_t>(sms) * 8 ? want : static_cast<size_t>(sms) * 8);
+    // a block: as many neighbouring pieces of a row as there are, up to 256, and rows for the rest of its threads
+    const size_t pieces = (cols + 16 / es - 1) / (16 / es);
+    unsigned bx = 1;
+    while (bx < static_cast<unsigned>(kQbThreads) && bx < pieces) bx *= 2;
+    const unsigned by = kQbThreads / bx;
+    const size_t block_rows_at_once = static_cast<size_t>(by) * kDequantRows;
+    const size_t row_steps = (rows + block_rows_at_once - 1) / block_rows_at_once;
+    const dim3 grid(static_cast<unsigned>((pieces + bx - 1) / bx), static_cast<unsigned>(row_steps < 65535 ? row_steps : 65535));
     const long long scale_rows = static_cast<long long>(block_rows == kQb ? (rows + kQb - 1) / kQb : rows);
     const int shift = block_rows == kQb ? 7 : 0;
-    const int vec_in = aligned(q, ld_q, 8), vec_out = aligned(out, ld_out * es, 16);
+    const int vec_in = aligned(q, ld_q, 16 / es), vec_out = aligned(out, ld_out * es, 16);
     auto go = [&](auto kernel) {
-        return launch_pdl(kernel, dim3(blocks), dim3(kQbThreads), 0, stream, static_cast<const uint8_t*>(q),
+        return launch_pdl(kernel, grid, dim3(bx, by), 0, stream, static_cast<const uint8_t*>(q),
                           static_cast<long long>(ld_q), scale, shift, scale_rows, static_cast<int>(rows),
                           static_cast<int>(cols), static_cast<uint8_t*>(out), static_cast<long long>(ld_out), vec_in, vec_out);
     };

@@ -102,11 +102,38 @@ def test_quantize_block_empty(qlib, dev):
 
 
 @pytest.mark.parametrize("rows,cols", SIZES + [(640, 384)])
-def test_requantize_block_is_exact(qlib, dev, rows, cols):
-    q, s = qlib.quantize_block(_data(rows, cols, torch.float32, dev, 3 * rows + cols, 8.0))
+@pytest.mark.parametrize("spread", [0.5, 3.0, 8.0])
+def test_requantize_block_is_exact(qlib, dev, rows, cols, spread):
+    """Rows near one another, at the limit of fp16 arithmetic (2^15 apart), and far beyond it."""
+    q, s = qlib.quantize_block(_data(rows, cols, torch.float32, dev, 3 * rows + cols, spread))
     qt_ref, st_ref = quantize(values(q, s).t())
     qt, st = qlib.requantize_block(q, s)
     assert torch.equal(bytes_of(st), st_ref) and torch.equal(bytes_of(qt), qt_ref)
+
+
+@pytest.mark.parametrize("shift", [0, 1, 14, 15, 16, 17])
+@pytest.mark.parametrize("base", [0, 16, 120, 238])
+def test_requantize_block_at_the_edges(qlib, dev, base, shift):
+    """Scales exactly `shift` powers of two apart down to the smallest and up to the largest byte; columns of zeros, of
+    the smallest codes alone, of 448 and next to it, of negative zeros, and one NaN code."""
+    g = torch.Generator().manual_seed(7)
+    codes = torch.randint(0, 256, (300, 400), generator=g, dtype=torch.uint8)
+    codes[codes & 0x7F == 0x7F] = 0x7E
+    codes[:, 5] = 0
+    codes[:, 6] = 0x80
+    codes[:, 7] = torch.randint(0, 2, (300,), generator=g, dtype=torch.uint8)  # 0 or 2^-9
+    codes[:, 8] = 0x01
+    codes[:, 9] = 0x08  # 2^-6
+    codes[:, 10] = 0x07
+    codes[:, 130] = 0xFE
+    codes[3:9] = 0
+    codes[200, 390] = 0x7F
+    scale = (base + torch.randint(0, shift + 1, (4, 300), generator=g)).clamp(max=254).to(torch.uint8)
+    scale[:, 0], scale[:, 1] = base, min(base + shift, 254)
+    qt_ref, st_ref = quantize(values(codes, scale).t())
+    qt, st = qlib.requantize_block(codes.to(dev).view(E4M3), scale.to(dev).view(E8M0))
+    assert torch.equal(bytes_of(st), st_ref)
+    assert torch.equal(bytes_of(qt), qt_ref)
 
 
 def test_requantize_and_dequantize_every_code_and_scale(qlib, dev):
