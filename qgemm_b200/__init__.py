@@ -127,19 +127,30 @@ def _check(status: int, what: str) -> None:
 
 
 # ----------------------------------------------------------------------------- torch-level API
+_torch_module = None
+_dtype_table = None
+
+
 def _torch():
-    import torch
-    return torch
+    global _torch_module
+    if _torch_module is None:
+        import torch
+        _torch_module = torch
+    return _torch_module
 
 
 def _dtype_code(t) -> int:
-    torch = _torch()
-    table = {torch.bfloat16: BF16, torch.float16: FP16, torch.int8: INT8, torch.float32: FP32, torch.int32: INT32}
-    if hasattr(torch, "float8_e4m3fn"):
-        table[torch.float8_e4m3fn] = FP8_E4M3
-    if t.dtype not in table:
+    global _dtype_table
+    if _dtype_table is None:
+        torch = _torch()
+        table = {torch.bfloat16: BF16, torch.float16: FP16, torch.int8: INT8, torch.float32: FP32, torch.int32: INT32}
+        if hasattr(torch, "float8_e4m3fn"):
+            table[torch.float8_e4m3fn] = FP8_E4M3
+        _dtype_table = table
+    code = _dtype_table.get(t.dtype)
+    if code is None:
         raise QgemmError(ERR_UNSUPPORTED, f"dtype {t.dtype}")
-    return table[t.dtype]
+    return code
 
 
 def _require_cuda_2d(name, t):
@@ -320,62 +331,102 @@ def fp8_block_mm(a, b, a_scale, b_scale, c, reference_layout: bool = True) -> No
 BLOCK = 128  #: elements of the summed axis that share a scale
 
 
-def _blocks(n: int) -> int:
-    return -(-n // BLOCK)
+def _invalid(what: str):
+    raise QgemmError(ERR_INVALID_ARG, what)
 
 
-def _same_device(what, *tensors):
-    if any(t.device != tensors[0].device for t in tensors):
-        raise QgemmError(ERR_INVALID_ARG, f"{what}: the tensors are on different devices")
-
-
-def _codes_empty(rows: int, cols: int, device):
-    """[rows, cols] e4m3 codes whose rows start on 16-byte boundaries, as the product reads them."""
+def _launch(name: str, device, *args) -> None:
+    """Calls the C entry ``name`` with ``args`` and the current stream of ``device``, on that device. These calls are short
+    (a few microseconds of GPU work when a token is generated), so the device is only switched when it has to be."""
     torch = _torch()
-    return torch.empty((rows, -(-cols // 16) * 16), dtype=torch.float8_e4m3fn, device=device)[:, :cols]
+    index = device.index
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    fn = getattr(_lib or lib(), name)
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, stream)
+    if rc != OK:
+        raise QgemmError(rc, name)
 
 
-def _scale_block_rows(what: str, scale, rows: int, cols: int) -> int:
+def _matrix(name: str, t):
+    """(rows, cols, leading dimension) of a CUDA matrix with unit inner stride whose rows do not overlap. One row has no
+    leading dimension of its own: a multiple of 16, so that it asks for no alignment beyond its start's."""
+    if not t.is_cuda:
+        _invalid(f"{name} must be a CUDA tensor (there is no CPU path)")
+    if t.dim() != 2:
+        _invalid(f"{name} must be 2-D with unit inner stride")
+    rows, cols = t.shape
+    ld, inner = t.stride()
+    if inner != 1 and cols > 1:
+        _invalid(f"{name} must be 2-D with unit inner stride")
+    if rows <= 1:
+        return rows, cols, -(-max(ld, cols) // 16) * 16
+    if ld < cols:
+        _invalid(f"{name}: its rows overlap")
+    return rows, cols, ld
+
+
+def _codes(name: str, t):
+    if t.dtype != _torch().float8_e4m3fn:
+        _invalid(f"{name} must be float8_e4m3fn")
+    return _matrix(name, t)
+
+
+def _scale_block_rows(what: str, scale, rows: int, cols: int, device) -> int:
     """1 or 128: how many rows of a row-form [rows, cols] matrix share one of ``scale``'s entries, by its shape."""
+    if scale.dtype != _torch().float8_e8m0fnu or not scale.is_contiguous():
+        _invalid(f"{what} must be a contiguous float8_e8m0fnu CUDA tensor")
+    if scale.device != device:
+        _invalid(f"{what} is on another device than its codes")
+    blocks = -(-cols // BLOCK)
+    shape = tuple(scale.shape)
+    if shape == (blocks, rows):
+        return 1
+    if shape == (blocks, -(-rows // BLOCK)):
+        return BLOCK
+    _invalid(f"{what} of a [{rows}, {cols}] matrix is [{blocks}, {rows}] or [{blocks}, {-(-rows // BLOCK)}], got {list(shape)}")
+
+
+def _new_form(rows: int, cols: int, square: bool, device):
+    """Codes [rows, cols] whose rows start on 16-byte boundaries, as the product reads them, their leading dimension, and
+    their scales."""
     torch = _torch()
-    if not scale.is_cuda or scale.dtype != torch.float8_e8m0fnu or not scale.is_contiguous():
-        raise QgemmError(ERR_INVALID_ARG, f"{what} must be a contiguous float8_e8m0fnu CUDA tensor")
-    for block_rows, n in ((1, rows), (BLOCK, _blocks(rows))):
-        if tuple(scale.shape) == (_blocks(cols), n):
-            return block_rows
-    raise QgemmError(ERR_INVALID_ARG, f"{what} of a [{rows}, {cols}] matrix is [{_blocks(cols)}, {rows}] or "
-                     f"[{_blocks(cols)}, {_blocks(rows)}], got {list(scale.shape)}")
+    ld = -(-cols // 16) * 16
+    q = torch.empty((rows, ld), dtype=torch.float8_e4m3fn, device=device)
+    s = torch.empty((-(-cols // BLOCK), -(-rows // BLOCK) if square else rows), dtype=torch.float8_e8m0fnu, device=device)
+    return (q if ld == cols else q[:, :cols]), ld, s
 
 
-def _require_codes(name, t, rows=None, cols=None):
-    torch = _torch()
-    _require_cuda_2d(name, t)
-    if t.dtype != torch.float8_e4m3fn or (rows is not None and tuple(t.shape) != (rows, cols)):
-        raise QgemmError(ERR_INVALID_ARG, f"{name} must be float8_e4m3fn" + (f" [{rows}, {cols}]" if rows is not None else ""))
-
-
-def _ld(t) -> int:
-    """Leading dimension of a 2-D tensor with unit inner stride; one row has none of its own."""
-    if t.shape[0] <= 1:
-        return -(-max(t.stride(0), t.shape[1]) // 16) * 16
-    return t.stride(0)
-
-
-def _code_form(form_rows: int, form_cols: int, square: bool, out, what: str, device):
-    """(codes, scales) of one form, allocated or checked."""
-    torch = _torch()
-    shape = (_blocks(form_cols), _blocks(form_rows) if square else form_rows)
-    if out is None:
-        return _codes_empty(form_rows, form_cols, device), torch.empty(shape, dtype=torch.float8_e8m0fnu, device=device)
+def _given_form(out, rows: int, cols: int, square: bool, what: str, device):
     q, s = out
-    _require_codes(f"{what} codes", q, form_rows, form_cols)
-    if not s.is_cuda or s.dtype != torch.float8_e8m0fnu or tuple(s.shape) != shape or not s.is_contiguous():
-        raise QgemmError(ERR_INVALID_ARG, f"{what} scales must be a contiguous float8_e8m0fnu CUDA tensor {list(shape)}")
-    if q.device != device or s.device != device:
-        raise QgemmError(ERR_INVALID_ARG, f"{what}: the tensors are on different devices")
-    if form_rows > 1 and q.stride(0) < form_cols:
-        raise QgemmError(ERR_INVALID_ARG, f"{what} codes: rows overlap")
-    return q, s
+    r, c, ld = _codes(f"{what} codes", q)
+    if (r, c) != (rows, cols) or q.device != device:
+        _invalid(f"{what} codes are [{rows}, {cols}] on the source's device")
+    if _scale_block_rows(f"{what} scales", s, rows, cols, device) != (BLOCK if square and rows > 1 else 1):
+        _invalid(f"{what} scales: one for each {'square' if square else 'row'} of 128")
+    return q, ld, s
+
+
+def _quantize_block(x, rows: int, cols: int, ld: int, square: bool, row: bool, column: bool):
+    """:func:`quantize_block` of an already checked matrix, into new tensors."""
+    device = x.device
+    res = ()
+    qp = sp = qtp = stp = None
+    qld = qtld = 0
+    if row:
+        q, qld, s = _new_form(rows, cols, square, device)
+        qp, sp = q.data_ptr(), s.data_ptr()
+        res += (q, s)
+    if column:
+        q, qtld, s = _new_form(cols, rows, square, device)
+        qtp, stp = q.data_ptr(), s.data_ptr()
+        res += (q, s)
+    _launch("qgemm_quantize_block", device, _dtype_code(x), x.data_ptr(), ld, rows, cols, BLOCK if square else 1, qp, qld, sp,
+            qtp, qtld, stp)
+    return res
 
 
 def quantize_block(x, square: bool = False, form: str = "row", out=None):
@@ -391,77 +442,57 @@ def quantize_block(x, square: bool = False, form: str = "row", out=None):
     block holding an infinity or a NaN becomes NaN as a whole. New codes get rows that start on 16-byte boundaries (the
     product asks for that); ``out`` takes the tensors of an earlier call to write into instead."""
     torch = _torch()
-    _require_cuda_2d("x", x)
+    rows, cols, ld = _matrix("x", x)
     if form not in ("row", "column", "both"):
-        raise QgemmError(ERR_INVALID_ARG, f"form is 'row', 'column' or 'both', got {form!r}")
+        _invalid(f"form is 'row', 'column' or 'both', got {form!r}")
     if x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
         raise QgemmError(ERR_UNSUPPORTED, f"quantize_block of dtype {x.dtype}")
-    rows, cols = x.shape
-    if rows > 1 and x.stride(0) < cols:
-        raise QgemmError(ERR_INVALID_ARG, "quantize_block: the rows of x overlap")
+    row, column = form != "column", form != "row"
+    if out is None:
+        return _quantize_block(x, rows, cols, ld, square, row, column)
     n = 4 if form == "both" else 2
-    if out is not None and len(out) != n:
-        raise QgemmError(ERR_INVALID_ARG, f"out has {n} tensors with form={form!r}")
-    res = ()
-    q = s = qt = st = None
-    if form != "column":
-        q, s = _code_form(rows, cols, square, None if out is None else out[:2], "row form", x.device)
-        res += (q, s)
-    if form != "row":
-        qt, st = _code_form(cols, rows, square, None if out is None else out[-2:], "column form", x.device)
-        res += (qt, st)
-    with torch.cuda.device(x.device):
-        rc = lib().qgemm_quantize_block(
-            _dtype_code(x), x.data_ptr(), _ld(x), rows, cols, BLOCK if square else 1,
-            q.data_ptr() if q is not None else None, _ld(q) if q is not None else 0, s.data_ptr() if s is not None else None,
-            qt.data_ptr() if qt is not None else None, _ld(qt) if qt is not None else 0,
-            st.data_ptr() if st is not None else None, _stream_ptr(x))
-    _check(rc, "qgemm_quantize_block")
-    return res
+    if len(out) != n:
+        _invalid(f"out has {n} tensors with form={form!r}")
+    args = [None, 0, None, None, 0, None]
+    if row:
+        q, qld, s = _given_form(out[:2], rows, cols, square, "row form", x.device)
+        args[:3] = q.data_ptr(), qld, s.data_ptr()
+    if column:
+        q, qld, s = _given_form(out[-2:], cols, rows, square, "column form", x.device)
+        args[3:] = q.data_ptr(), qld, s.data_ptr()
+    _launch("qgemm_quantize_block", x.device, _dtype_code(x), x.data_ptr(), ld, rows, cols, BLOCK if square else 1, *args)
+    return tuple(out)
 
 
 def requantize_block(q, scale, out=None):
     """Column form ``(qt, scale_t)`` of a matrix held in row form with a scale per row and block: the values
     code * scale quantised anew over blocks of 128 rows. Turns a saved 8-bit activation into the operand of the weight
     gradient, dW = dy^T x. (A matrix with ``square`` scales needs no new codes: transpose codes and scales.)"""
-    torch = _torch()
-    _require_codes("q", q)
-    rows, cols = q.shape
-    if rows > 1 and q.stride(0) < cols:
-        raise QgemmError(ERR_INVALID_ARG, "requantize_block: the rows of q overlap")
-    if _scale_block_rows("scale", scale, rows, cols) != 1:
+    rows, cols, ld = _codes("q", q)
+    if _scale_block_rows("scale", scale, rows, cols, q.device) != 1:
         raise QgemmError(ERR_UNSUPPORTED, "requantize_block takes a scale per row; with square blocks transpose codes and scales")
-    _same_device("requantize_block", q, scale)
-    qt, st = _code_form(cols, rows, False, out, "column form", q.device)
-    with torch.cuda.device(q.device):
-        rc = lib().qgemm_requantize_block(q.data_ptr(), _ld(q), scale.data_ptr(), rows, cols, qt.data_ptr(), _ld(qt),
-                                          st.data_ptr(), _stream_ptr(q))
-    _check(rc, "qgemm_requantize_block")
+    if out is None:
+        qt, ldt, st = _new_form(cols, rows, False, q.device)
+    else:
+        qt, ldt, st = _given_form(out, cols, rows, False, "column form", q.device)
+    _launch("qgemm_requantize_block", q.device, q.data_ptr(), ld, scale.data_ptr(), rows, cols, qt.data_ptr(), ldt, st.data_ptr())
     return qt, st
 
 
 def dequantize_block(q, scale, out_dtype=None, out=None):
     """code * scale of a row-form matrix, rounded to ``out_dtype`` (bf16 unless told otherwise; fp16, fp32)."""
     torch = _torch()
-    _require_codes("q", q)
-    rows, cols = q.shape
-    if rows > 1 and q.stride(0) < cols:
-        raise QgemmError(ERR_INVALID_ARG, "dequantize_block: the rows of q overlap")
-    block_rows = _scale_block_rows("scale", scale, rows, cols)
+    rows, cols, ld = _codes("q", q)
+    block_rows = _scale_block_rows("scale", scale, rows, cols, q.device)
     if out is None:
         out = torch.empty((rows, cols), dtype=out_dtype or torch.bfloat16, device=q.device)
-    _require_cuda_2d("out", out)
-    if tuple(out.shape) != (rows, cols) or (out_dtype is not None and out.dtype != out_dtype):
-        raise QgemmError(ERR_INVALID_ARG, "out must have q's shape and the requested dtype")
     if out.dtype not in (torch.bfloat16, torch.float16, torch.float32):
         raise QgemmError(ERR_UNSUPPORTED, f"dequantize_block to dtype {out.dtype}")
-    if rows > 1 and out.stride(0) < cols:
-        raise QgemmError(ERR_INVALID_ARG, "dequantize_block: the rows of out overlap")
-    _same_device("dequantize_block", q, scale, out)
-    with torch.cuda.device(q.device):
-        rc = lib().qgemm_dequantize_block(_dtype_code(out), q.data_ptr(), _ld(q), scale.data_ptr(), block_rows, rows, cols,
-                                          out.data_ptr(), _ld(out), _stream_ptr(q))
-    _check(rc, "qgemm_dequantize_block")
+    r, c, ldo = _matrix("out", out)
+    if (r, c) != (rows, cols) or (out_dtype is not None and out.dtype != out_dtype) or out.device != q.device:
+        _invalid("out must have q's shape and device and the requested dtype")
+    _launch("qgemm_dequantize_block", q.device, _dtype_code(out), q.data_ptr(), ld, scale.data_ptr(), block_rows, rows, cols,
+            out.data_ptr(), ldo)
     return out
 
 
@@ -471,24 +502,18 @@ def fp8_block_mm_e8m0(a, b, a_scale, b_scale, c, accumulate: bool = False) -> No
     [ceil(k/128), ceil(m/128)]; ``b_scale`` likewise of n. ``c`` bf16 / fp16 / fp32; ``accumulate`` adds to what a fp32 ``c``
     holds. Rows of ``a`` and ``b`` start on 16-byte boundaries. A layer's three products, with x, w and dy quantised:
     forward (x row, w row), dx = (dy row, w column), dw = (dy column, x column)."""
-    torch = _torch()
-    _require_codes("a", a)
-    _require_codes("b", b)
-    _require_cuda_2d("c", c)
-    M, K = a.shape
-    N = b.shape[0]
-    if b.shape[1] != K or tuple(c.shape) != (M, N):
-        raise QgemmError(ERR_INVALID_ARG, f"shape mismatch a{tuple(a.shape)} b{tuple(b.shape)} c{tuple(c.shape)}")
-    a_rows = _scale_block_rows("a_scale", a_scale, M, K)
-    b_rows = _scale_block_rows("b_scale", b_scale, N, K)
-    _same_device("fp8_block_mm_e8m0", a, b, a_scale, b_scale, c)
-    if M > 1 and c.stride(0) < N:
-        raise QgemmError(ERR_INVALID_ARG, "the rows of c overlap")
-    with torch.cuda.device(a.device):
-        rc = lib().qgemm_fp8_block_e8m0_gemm(
-            _dtype_code(c), a.data_ptr(), _ld(a), a_scale.data_ptr(), a_rows, b.data_ptr(), _ld(b), b_scale.data_ptr(), b_rows,
-            1 if accumulate else 0, c.data_ptr(), _ld(c), M, N, K, _stream_ptr(a))
-    _check(rc, "qgemm_fp8_block_e8m0_gemm")
+    M, K, lda = _codes("a", a)
+    N, Kb, ldb = _codes("b", b)
+    rows, cols, ldc = _matrix("c", c)
+    device = a.device
+    if Kb != K or rows != M or cols != N:
+        _invalid(f"shape mismatch a{tuple(a.shape)} b{tuple(b.shape)} c{tuple(c.shape)}")
+    if b.device != device or c.device != device:
+        _invalid("fp8_block_mm_e8m0: the tensors are on different devices")
+    a_rows = _scale_block_rows("a_scale", a_scale, M, K, device)
+    b_rows = _scale_block_rows("b_scale", b_scale, N, K, device)
+    _launch("qgemm_fp8_block_e8m0_gemm", device, _dtype_code(c), a.data_ptr(), lda, a_scale.data_ptr(), a_rows, b.data_ptr(),
+            ldb, b_scale.data_ptr(), b_rows, 1 if accumulate else 0, c.data_ptr(), ldc, M, N, K)
 
 
 MAX_DSTS = 8  # QGEMM_MAX_DSTS

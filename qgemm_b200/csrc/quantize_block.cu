@@ -341,9 +341,17 @@ __device__ __forceinline__ bool whole_tile(const QuantBlockParams& p) {
            static_cast<int>(blockIdx.x + 1) * kQb <= p.cols;
 }
 
-// Both forms of a 16-bit matrix would take 100 registers, two tiles an SM: held to three (4096 x 7168 25.9 -> 22.3 us).
+// Tiles that share an SM, by the registers a tile can be held in: what a CTA has in flight is its tile, so this sets the
+// bandwidth. (16-bit, 4096 x 7168, column form: four 16.4 us,
+// two 21.3, five, with spilled registers, 18.7; both forms: three 22.3, two 25.9, four 23.2.)
 template <typename T, bool ROW, bool COL, bool SQUARE>
-__global__ void __launch_bounds__(kQbThreads, ROW && COL && !SQUARE && sizeof(typename Elem<T>::type) == 2 ? 3 : 1)
+constexpr int tiles_per_sm() {
+    if (sizeof(typename Elem<T>::type) == 2) return SQUARE ? (ROW ? 4 : 5) : (ROW && COL ? 3 : 4);
+    return ROW ? 2 : 3;
+}
+
+template <typename T, bool ROW, bool COL, bool SQUARE>
+__global__ void __launch_bounds__(kQbThreads, (tiles_per_sm<T, ROW, COL, SQUARE>()))
 quantize_block_kernel(const QuantBlockParams p) {
     ptx::pdl_launch_dependents();
     ptx::pdl_wait();

@@ -16,11 +16,12 @@ c)`` (src/mix_gemm/hip_mix_gemm_kernel.cpp:508-516) is the forward product alone
 """
 from __future__ import annotations
 
+from contextlib import nullcontext
 from dataclasses import dataclass
 
 import torch
 
-from . import ERR_INVALID_ARG, ERR_UNSUPPORTED, QgemmError, fp8_block_mm_e8m0, quantize_block, requantize_block
+from . import ERR_INVALID_ARG, ERR_UNSUPPORTED, QgemmError, _matrix, _quantize_block, fp8_block_mm_e8m0, requantize_block
 
 _TYPES = (torch.bfloat16, torch.float16, torch.float32)
 
@@ -61,8 +62,13 @@ def pack_weight(weight, backward: bool = False) -> PackedWeight:
     with respect to x can be taken (the weight itself gets none)."""
     if weight.dim() != 2:
         raise QgemmError(ERR_INVALID_ARG, "a weight is [out, in]")
-    res = quantize_block(_rows(weight.detach()), square=True, form="both" if backward else "row")
-    return PackedWeight(*res)
+    if weight.dtype not in _TYPES:
+        raise QgemmError(ERR_UNSUPPORTED, f"a weight of dtype {weight.dtype}")
+    return PackedWeight(*_quantized(_rows(weight.detach()), True, True, backward))
+
+
+def _quantized(t, square: bool, row: bool, column: bool):
+    return _quantize_block(t, *_matrix("matrix", t), square, row, column)
 
 
 def _rows(t):
@@ -80,10 +86,18 @@ def _flat(x, features: int, what: str):
         raise QgemmError(ERR_INVALID_ARG, f"{what} must be a CUDA tensor (there is no CPU path)")
     if x.dtype not in _TYPES:
         raise QgemmError(ERR_UNSUPPORTED, f"{what} of dtype {x.dtype}")
+    if x.requires_grad:
+        x = x.detach()
+    if x.dim() != 2:
+        x = x.reshape(_tokens(x.shape), features)
+    return _rows(x)
+
+
+def _tokens(shape) -> int:
     tokens = 1
-    for d in x.shape[:-1]:
+    for d in shape[:-1]:
         tokens *= d
-    return _rows(x.reshape(tokens, features))
+    return tokens
 
 
 def fp8_linear_forward(x, weight, need_dx: bool = True, need_dw: bool = True, out_dtype=None):
@@ -95,7 +109,7 @@ def fp8_linear_forward(x, weight, need_dx: bool = True, need_dw: bool = True, ou
     if weight.device != x.device:
         raise QgemmError(ERR_INVALID_ARG, "x and the weight are on different devices")
     out_features, in_features = weight.shape
-    x2 = _flat(x.detach(), in_features, "x")
+    x2 = _flat(x, in_features, "x")
     if packed:
         if need_dw:
             raise QgemmError(ERR_INVALID_ARG, "a PackedWeight has no gradient: need_dw=False")
@@ -103,26 +117,24 @@ def fp8_linear_forward(x, weight, need_dx: bool = True, need_dw: bool = True, ou
             raise QgemmError(ERR_INVALID_ARG, "gradients with respect to x need pack_weight(..., backward=True)")
         w, ws, wt, wts = weight.codes, weight.scale, weight.codes_t, weight.scale_t
     else:
-        w, ws, *turned = quantize_block(_rows(weight.detach()), square=True, form="both" if need_dx else "row")
+        w, ws, *turned = _quantized(_rows(weight.detach()), True, True, need_dx)
         wt, wts = turned if turned else (None, None)
-    xq, xs = quantize_block(x2)
+    xq, xs = _quantized(x2, False, True, False)
     y = torch.empty((x2.shape[0], out_features), dtype=out_dtype or x.dtype, device=x.device)
     fp8_block_mm_e8m0(xq, w, xs, ws, y)
     saved = LinearSaved(xq if need_dw else None, xs if need_dw else None, wt if need_dx else None, wts if need_dx else None,
                         tuple(x.shape), x.dtype, None if packed else weight.dtype, out_features)
-    return y.view(*x.shape[:-1], out_features), saved
+    return (y if x.dim() == 2 else y.view(*x.shape[:-1], out_features)), saved
 
 
 def fp8_linear_backward(dy, saved: LinearSaved, dw=None, accumulate: bool = False):
     """``(dx, dw)`` from dy [..., out] and what the forward call saved; None for a gradient it saved nothing for. ``dw``: a
     matrix [out, in] to write into instead of a new one, or with ``accumulate`` (fp32) to add to, as over the micro-batches
     of one step."""
-    dy2 = _flat(dy.detach(), saved.out_features, "dy")
+    dy2 = _flat(dy, saved.out_features, "dy")
     in_features = saved.x_shape[-1]
     need_dx, need_dw = saved.weight_codes_t is not None, saved.x_codes is not None
-    tokens = 1
-    for d in saved.x_shape[:-1]:
-        tokens *= d
+    tokens = _tokens(saved.x_shape)
     if dy2.shape[0] != tokens:
         raise QgemmError(ERR_INVALID_ARG, f"dy has {dy2.shape[0]} rows, x had {tokens}")
     kept = saved.x_codes if need_dw else saved.weight_codes_t
@@ -134,7 +146,7 @@ def fp8_linear_backward(dy, saved: LinearSaved, dw=None, accumulate: bool = Fals
         raise QgemmError(ERR_INVALID_ARG, "the forward call saved nothing for dw")
     if not need_dx and not need_dw:
         return None, None
-    forms = quantize_block(dy2, form="both" if need_dx and need_dw else ("row" if need_dx else "column"))
+    forms = _quantized(dy2, False, need_dx, need_dw)
     dx = None
     if need_dx:
         dx = torch.empty((tokens, in_features), dtype=saved.x_dtype, device=dy.device)
@@ -190,7 +202,7 @@ def fp8_linear(x, weight, out_dtype=None):
     if not x.is_cuda:
         raise QgemmError(ERR_INVALID_ARG, "x must be a CUDA tensor (there is no CPU path)")
     stream = torch.cuda.current_stream(x.device).cuda_stream
-    with torch.cuda.device(x.device):
+    with nullcontext() if torch.cuda.current_device() == x.device.index else torch.cuda.device(x.device):
         capturing = torch.cuda.is_current_stream_capturing()
     if capturing and any(n.metadata.get(_STREAM, stream) != stream for n in _accumulators(x, w)):
         raise QgemmError(ERR_UNSUPPORTED, "capturing a graph while an earlier graph of the same leaves is alive")
