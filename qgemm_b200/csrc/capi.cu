@@ -118,14 +118,8 @@ std::unordered_map<MapKey, CUtensorMap, MapKeyHash> g_maps;
 // 128-byte swizzle, zero fill outside the tensor. kgroup > 1 (cols a whole number of 128-byte blocks): the
 // three-dimensional view [128 bytes][rows][K blocks] with a box of kgroup K blocks, which lands in shared memory as
 // kgroup consecutive [box_rows][128 bytes] tiles (see GemmParams::kgroup).
-int make_operand_map(const void* ptr, uint64_t rows, uint64_t cols, uint64_t ld, int in_dtype, uint32_t box_rows,
-                     CUtensorMap* out, uint32_t kgroup = 1) {
-    const MapKey key{ptr, rows, cols, ld, box_rows, static_cast<uint32_t>(in_dtype) + 1000u * kgroup};
-    auto it = g_maps.find(key);
-    if (it != g_maps.end()) {
-        *out = it->second;
-        return QGEMM_OK;
-    }
+int encode_operand_map(const void* ptr, uint64_t rows, uint64_t cols, uint64_t ld, int in_dtype, uint32_t box_rows,
+                       CUtensorMap* out, uint32_t kgroup = 1) {
     CUtensorMapDataType dt;
     uint32_t es;
     switch (in_dtype) {
@@ -151,22 +145,29 @@ int make_operand_map(const void* ptr, uint64_t rows, uint64_t cols, uint64_t ld,
                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     }
     if (r != CUDA_SUCCESS) return QGEMM_ERR_CUDA;
-    if (g_maps.size() > 4096) g_maps.clear();
-    g_maps.emplace(key, m);
     *out = m;
+    return QGEMM_OK;
+}
+
+int make_operand_map(const void* ptr, uint64_t rows, uint64_t cols, uint64_t ld, int in_dtype, uint32_t box_rows,
+                     CUtensorMap* out, uint32_t kgroup = 1) {
+    const MapKey key{ptr, rows, cols, ld, box_rows, static_cast<uint32_t>(in_dtype) + 1000u * kgroup};
+    auto it = g_maps.find(key);
+    if (it != g_maps.end()) {
+        *out = it->second;
+        return QGEMM_OK;
+    }
+    const int rc = encode_operand_map(ptr, rows, cols, ld, in_dtype, box_rows, out, kgroup);
+    if (rc != QGEMM_OK) return rc;
+    if (g_maps.size() > 4096) g_maps.clear();
+    g_maps.emplace(key, *out);
     return QGEMM_OK;
 }
 
 // Output [splits][M][N] (splits == 1 for the final C) with leading dimension ld and slab stride
 // M*ld, elements of 2 or 4 bytes; box = 128 bytes of N x 32 rows x 1 slab, 128-byte swizzle. Stores
 // through it are clipped at N, at M (per slab) and at the slab count.
-int make_output_map(void* ptr, uint64_t M, uint64_t N, uint64_t ld, uint64_t splits, int out_kind, CUtensorMap* out) {
-    const MapKey key{ptr, M, N, ld, static_cast<uint32_t>(splits), static_cast<uint32_t>(100 + out_kind)};
-    auto it = g_maps.find(key);
-    if (it != g_maps.end()) {
-        *out = it->second;
-        return QGEMM_OK;
-    }
+int encode_output_map(void* ptr, uint64_t M, uint64_t N, uint64_t ld, uint64_t splits, int out_kind, CUtensorMap* out) {
     CUtensorMapDataType dt;
     uint32_t es;
     switch (out_kind) {
@@ -184,9 +185,21 @@ int make_output_map(void* ptr, uint64_t M, uint64_t N, uint64_t ld, uint64_t spl
                                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return QGEMM_ERR_CUDA;
-    if (g_maps.size() > 4096) g_maps.clear();
-    g_maps.emplace(key, m);
     *out = m;
+    return QGEMM_OK;
+}
+
+int make_output_map(void* ptr, uint64_t M, uint64_t N, uint64_t ld, uint64_t splits, int out_kind, CUtensorMap* out) {
+    const MapKey key{ptr, M, N, ld, static_cast<uint32_t>(splits), static_cast<uint32_t>(100 + out_kind)};
+    auto it = g_maps.find(key);
+    if (it != g_maps.end()) {
+        *out = it->second;
+        return QGEMM_OK;
+    }
+    const int rc = encode_output_map(ptr, M, N, ld, splits, out_kind, out);
+    if (rc != QGEMM_OK) return rc;
+    if (g_maps.size() > 4096) g_maps.clear();
+    g_maps.emplace(key, *out);
     return QGEMM_OK;
 }
 
@@ -1077,6 +1090,40 @@ int blockscale_dispatch(int out_dtype, int a_layout, int b_layout, const void* A
     return launch_fp8_blockscale(out_kind, ta, tb, tc, p, grid, stream) == cudaSuccess ? QGEMM_OK : QGEMM_ERR_CUDA;
 }
 
+// One launch of the power-of-two block-scaled GEMM in a given form. `p` has the matrices' addresses, leading dimensions and
+// sizes; the rest is filled in here.
+int e8m0_launch(const E8m0Plan& plan, const void* A, size_t lda, const void* B, size_t ldb, E8m0Params p, int sms,
+                cudaStream_t stream) {
+    const size_t out_bytes = (p.out == OUT_F32) ? 4 : 2;
+    const uintptr_t c_addr = reinterpret_cast<uintptr_t>(p.C);
+    p.kb_total = (p.K + 127) / 128;
+    p.c_vec_ok = c_addr % (4 * out_bytes) == 0 && p.ldc % 4 == 0;
+    p.m_tiles = (p.M + plan.tile_m - 1) / plan.tile_m;
+    p.n_tiles = (p.N + plan.tile_n - 1) / plan.tile_n;
+    const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
+    if (tiles * 8 > 0x7fffffffLL) return QGEMM_ERR_UNSUPPORTED;
+    CUtensorMap ta, tb, tc;
+    int rc = encode_operand_map(A, p.M, p.K, lda, QGEMM_DTYPE_FP8_E4M3, static_cast<uint32_t>(std::min(plan.tile_m, 128)), &ta);
+    if (rc != QGEMM_OK) return rc;
+    const uint32_t b_box = plan.tile_m == 256 ? static_cast<uint32_t>(plan.tile_n / 2) : 128u;  // a pair's CTAs load half each
+    rc = encode_operand_map(B, p.N, p.K, ldb, QGEMM_DTYPE_FP8_E4M3, b_box, &tb);
+    if (rc != QGEMM_OK) return rc;
+    if (plan.tile_m != 256) {
+        p.idesc = ptx::make_idesc_e8m0(128u, static_cast<uint32_t>(plan.tile_m));
+        return launch_e8m0_small(plan.tile_m, plan.slices, ta, tb, p, stream) == cudaSuccess ? QGEMM_OK : QGEMM_ERR_CUDA;
+    }
+    std::memset(&tc, 0, sizeof(tc));
+    if (c_addr % 16 == 0 && (static_cast<size_t>(p.ldc) * out_bytes) % 16 == 0 && g_env.direct_store == 0)
+        p.c_tma_ok = encode_output_map(p.C, p.M, p.N, p.ldc, 1, p.out, &tc) == QGEMM_OK ? 1 : 0;
+    // tile rows walked together, so that their panels of A (16 MB of them) stay in L2 while B passes
+    p.group_m = g_env.group_m > 0
+                    ? g_env.group_m
+                    : static_cast<int>(std::max<long long>(4, std::min<long long>(4096, (16ll << 20) / (128ll * p.kb_total * 256))));
+    p.idesc = ptx::make_idesc_e8m0(256u, static_cast<uint32_t>(plan.tile_n));
+    const int clusters = static_cast<int>(std::min<long long>(tiles, sms / 2));
+    return launch_e8m0_pair(plan.tile_n, plan.slices, ta, tb, tc, p, clusters, stream) == cudaSuccess ? QGEMM_OK : QGEMM_ERR_CUDA;
+}
+
 // FP8 GEMM with power-of-two block scales. No library scratch: calls on different streams are independent.
 int e8m0_dispatch(int out_dtype, const void* A, size_t lda, const uint8_t* a_scale, int a_block_rows, const void* B,
                   size_t ldb, const uint8_t* b_scale, int b_block_rows, int accumulate, void* C, size_t ldc, size_t M,
@@ -1101,7 +1148,7 @@ int e8m0_dispatch(int out_dtype, const void* A, size_t lda, const uint8_t* a_sca
 
     std::lock_guard<std::mutex> lock(g_mutex);
     DeviceState* st = nullptr;
-    int rc = get_state(&st);
+    const int rc = get_state(&st);
     if (rc != QGEMM_OK) return rc;
 
     E8m0Params p;
@@ -1111,7 +1158,6 @@ int e8m0_dispatch(int out_dtype, const void* A, size_t lda, const uint8_t* a_sca
     p.M = static_cast<int>(M);
     p.N = static_cast<int>(N);
     p.K = static_cast<int>(K);
-    p.kb_total = static_cast<int>((K + 127) / 128);
     p.a_scale = a_scale;
     p.b_scale = b_scale;
     p.a_shift = a_block_rows == 128 ? 7 : 0;
@@ -1121,32 +1167,8 @@ int e8m0_dispatch(int out_dtype, const void* A, size_t lda, const uint8_t* a_sca
     p.out = out_kind;
     p.accumulate = accumulate != 0;
     p.status = st->status;
-    p.c_vec_ok = reinterpret_cast<uintptr_t>(C) % (4 * out_bytes) == 0 && ldc % 4 == 0;
 
-    const E8m0Plan plan = plan_e8m0(M, N, K, st->sm_count);
-    CUtensorMap ta, tb, tc;
-    p.m_tiles = static_cast<int>((M + plan.tile_m - 1) / plan.tile_m);
-    p.n_tiles = static_cast<int>((N + plan.tile_n - 1) / plan.tile_n);
-    if (static_cast<long long>(p.m_tiles) * p.n_tiles * 8 > 0x7fffffffLL) return QGEMM_ERR_UNSUPPORTED;
-    rc = make_operand_map(A, M, K, lda, QGEMM_DTYPE_FP8_E4M3, static_cast<uint32_t>(std::min(plan.tile_m, 128)), &ta);
-    if (rc != QGEMM_OK) return rc;
-    const uint32_t b_box = plan.tile_m == 256 ? static_cast<uint32_t>(plan.tile_n / 2) : 128u;  // a pair's CTAs load half each
-    rc = make_operand_map(B, N, K, ldb, QGEMM_DTYPE_FP8_E4M3, b_box, &tb);
-    if (rc != QGEMM_OK) return rc;
-    if (plan.tile_m == 256) {  // CTA pairs
-        std::memset(&tc, 0, sizeof(tc));
-        if (reinterpret_cast<uintptr_t>(C) % 16 == 0 && (ldc * out_bytes) % 16 == 0 && g_env.direct_store == 0)
-            p.c_tma_ok = make_output_map(C, M, N, ldc, 1, out_kind, &tc) == QGEMM_OK ? 1 : 0;
-        // tile rows walked together, so that their panels of A (16 MB of them) stay in L2 while B passes
-        p.group_m = g_env.group_m > 0
-                        ? g_env.group_m
-                        : static_cast<int>(std::max<long long>(4, std::min<long long>(4096, (16ll << 20) / (128ll * p.kb_total * 256))));
-        p.idesc = ptx::make_idesc_e8m0(256u, static_cast<uint32_t>(plan.tile_n));
-        const int clusters = static_cast<int>(std::min<long long>(static_cast<long long>(p.m_tiles) * p.n_tiles, st->sm_count / 2));
-        return launch_e8m0_pair(plan.tile_n, plan.slices, ta, tb, tc, p, clusters, stream) == cudaSuccess ? QGEMM_OK : QGEMM_ERR_CUDA;
-    }
-    p.idesc = ptx::make_idesc_e8m0(128u, static_cast<uint32_t>(plan.tile_m));
-    return launch_e8m0_small(plan.tile_m, plan.slices, ta, tb, p, stream) == cudaSuccess ? QGEMM_OK : QGEMM_ERR_CUDA;
+    return e8m0_launch(plan_e8m0(M, N, K, st->sm_count), A, lda, B, ldb, p, st->sm_count, stream);
 }
 
 }  // namespace

@@ -192,65 +192,78 @@ __device__ __forceinline__ void e8_decode(int w, const E8m0Params& p, int& m_blk
 
 constexpr int kE8RowWords = 128 + 4;  // a row of 128 partial sums in shared memory, padded
 
+// Four sums to C[row][..]: columns n .. n + 3 as a vector, or (VEC false) those of n, n + 32, n + 64, n + 96 that exist.
+template <bool VEC>
+__device__ __forceinline__ void store_four(const E8m0Params& p, long long row, int n, const float (&acc)[4]) {
+    const long long at = row * p.ldc + n;
+    if (p.out == OUT_F32) {
+        float* dst = static_cast<float*>(p.C) + at;
+        if constexpr (VEC) {
+            float4 o = make_float4(acc[0], acc[1], acc[2], acc[3]);
+            if (p.accumulate) {
+                const float4 old = *reinterpret_cast<const float4*>(dst);
+                o = make_float4(old.x + o.x, old.y + o.y, old.z + o.z, old.w + o.w);
+            }
+            *reinterpret_cast<float4*>(dst) = o;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (n + 32 * j < p.N) dst[32 * j] = p.accumulate ? dst[32 * j] + acc[j] : acc[j];
+        }
+        return;
+    }
+    uint32_t u[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        if (p.out == OUT_BF16) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(acc[2 * j], acc[2 * j + 1]);
+            u[j] = *reinterpret_cast<const uint32_t*>(&h);
+        } else {
+            const __half2 h = __floats2half2_rn(acc[2 * j], acc[2 * j + 1]);
+            u[j] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+    }
+    uint16_t* dst = static_cast<uint16_t*>(p.C) + at;
+    if constexpr (VEC) {
+        *reinterpret_cast<uint2*>(dst) = make_uint2(u[0], u[1]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (n + 32 * j < p.N) dst[32 * j] = static_cast<uint16_t>((j & 1) ? (u[j >> 1] >> 16) : (u[j >> 1] & 0xffffu));
+    }
+}
+
 // Adds up the S partial tiles ([rows][kE8RowWords] fp32 at the start of the shared memory of cluster CTAs first, first + STEP,
 // ...) in that order and stores the sums to C[m0 ..][n0 .. n0 + 128]. The `rows` valid rows are dealt out over the S CTAs, of
-// which this is number `part`; a warp takes a row, a lane four columns.
+// which this is number `part`; a warp takes a row, a lane four columns: neighbouring ones where C takes vectors of four,
+// 32 apart where it does not, so that a warp's store is contiguous either way.
 template <int S, int STEP>
 __device__ __forceinline__ void sum_and_store(const E8m0Params& p, uint32_t smem_base, uint32_t first, uint32_t part, int m0,
                                               int rows, int n0) {
     const int warp = static_cast<int>(threadIdx.x) >> 5, lane = static_cast<int>(threadIdx.x) & 31;
     const int per = (rows + S - 1) / S;
     const int r1 = min(rows, (static_cast<int>(part) + 1) * per);
-    const int n = n0 + lane * 4;
-    const int n_valid = min(4, p.N - n);
-    if (n_valid <= 0) return;
-    const bool vec = p.c_vec_ok != 0 && n_valid == 4;
+    const bool vec = p.c_vec_ok != 0 && n0 + 128 <= p.N;
     for (int r = static_cast<int>(part) * per + warp; r < r1; r += kE8Threads / 32) {
-        const uint32_t own = smem_base + static_cast<uint32_t>((r * kE8RowWords + lane * 4) * 4);
+        const uint32_t row = smem_base + static_cast<uint32_t>(r * kE8RowWords * 4);
         float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         uint32_t w[S][4];
 #pragma unroll
         for (uint32_t k = 0; k < static_cast<uint32_t>(S); ++k) {
-            if constexpr (S > 1) ptx::ld_shared_cluster_v4(ptx::mapa_shared(own, first + k * STEP), w[k][0], w[k][1], w[k][2], w[k][3]);
-            else ptx::ld_shared_cluster_v4(own, w[k][0], w[k][1], w[k][2], w[k][3]);
+            const uint32_t at = S > 1 ? ptx::mapa_shared(row, first + k * STEP) : row;
+            if (vec) {
+                ptx::ld_shared_cluster_v4(at + lane * 16, w[k][0], w[k][1], w[k][2], w[k][3]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[k][j] = ptx::ld_shared_cluster_u32(at + (lane + 32 * j) * 4);
+            }
         }
 #pragma unroll
         for (int k = 0; k < S; ++k)
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[j] += __uint_as_float(w[k][j]);
-        const long long at = static_cast<long long>(m0 + r) * p.ldc + n;
-        if (p.out == OUT_F32) {
-            float* dst = static_cast<float*>(p.C) + at;
-            if (vec) {
-                float4 o = make_float4(acc[0], acc[1], acc[2], acc[3]);
-                if (p.accumulate) {
-                    const float4 old = *reinterpret_cast<const float4*>(dst);
-                    o = make_float4(old.x + o.x, old.y + o.y, old.z + o.z, old.w + o.w);
-                }
-                *reinterpret_cast<float4*>(dst) = o;
-            } else {
-                for (int j = 0; j < n_valid; ++j) dst[j] = p.accumulate ? dst[j] + acc[j] : acc[j];
-            }
-        } else {
-            uint32_t u[2];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                if (p.out == OUT_BF16) {
-                    const __nv_bfloat162 h = __floats2bfloat162_rn(acc[2 * j], acc[2 * j + 1]);
-                    u[j] = *reinterpret_cast<const uint32_t*>(&h);
-                } else {
-                    const __half2 h = __floats2half2_rn(acc[2 * j], acc[2 * j + 1]);
-                    u[j] = *reinterpret_cast<const uint32_t*>(&h);
-                }
-            }
-            uint16_t* dst = static_cast<uint16_t*>(p.C) + at;
-            if (vec) {
-                *reinterpret_cast<uint2*>(dst) = make_uint2(u[0], u[1]);
-            } else {
-                for (int j = 0; j < n_valid; ++j)
-                    dst[j] = static_cast<uint16_t>((j & 1) ? (u[j >> 1] >> 16) : (u[j >> 1] & 0xffffu));
-            }
-        }
+        if (vec) store_four<true>(p, m0 + r, n0 + lane * 4, acc);
+        else store_four<false>(p, m0 + r, n0 + lane, acc);
     }
 }
 
@@ -524,6 +537,35 @@ struct E8PairSmem {
     static_assert(kAccStep + BN <= kScaleCol && kScaleCol + kE8Cols * kScaleCols <= 512, "tensor-memory columns");
 };
 
+// A staged box to a C that TMA cannot address (any ldc, any base aligned to its element): a warp writes a row's 128 bytes
+// at a time, as words where the row starts on one. (Stored from registers, a row a lane, 2500 x 2500 x 8192 took 115 us.)
+template <int OUT>
+__device__ __forceinline__ void store_box_rows(const E8m0Params& p, uint32_t box, int row0, int n0, int lane) {
+    constexpr int OB = OutBytes<OUT>::value;
+    const int rows = min(32, p.M - row0);
+    uint8_t* dst = static_cast<uint8_t*>(p.C) + (static_cast<long long>(row0) * p.ldc + n0) * OB;
+    const long long step = p.ldc * OB;
+#pragma unroll 4
+    for (int r = 0; r < rows; ++r, dst += step) {
+        // 16-byte units of row r lie exchanged by r % 8
+        const uint32_t w = ptx::ld_shared_u32(box + static_cast<uint32_t>(r * 128 + (((lane >> 2) ^ (r & 7)) * 16) + (lane & 3) * 4));
+        if constexpr (OUT == OUT_F32) {
+            if (n0 + lane < p.N) {
+                float* f = reinterpret_cast<float*>(dst) + lane;
+                *f = p.accumulate ? *f + __uint_as_float(w) : __uint_as_float(w);
+            }
+        } else {
+            uint16_t* h = reinterpret_cast<uint16_t*>(dst) + 2 * lane;
+            if ((reinterpret_cast<uintptr_t>(dst) & 3u) == 0 && n0 + 64 <= p.N) {
+                *reinterpret_cast<uint32_t*>(h) = w;
+            } else {
+                if (n0 + 2 * lane < p.N) h[0] = static_cast<uint16_t>(w & 0xffffu);
+                if (n0 + 2 * lane + 1 < p.N) h[1] = static_cast<uint16_t>(w >> 16);
+            }
+        }
+    }
+}
+
 template <int OUT, int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kE8Threads, 1)
 gemm_e8m0_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
@@ -746,15 +788,15 @@ gemm_e8m0_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
                         }
                     }
                 }
-                if (p.c_tma_ok) {
-                    // the box is free once the store before has read it
-                    if (ptx::elect_one()) ptx::tma_store_wait_read<0>();
-                    __syncwarp();
-                    const uint32_t row_addr = stage_base + static_cast<uint32_t>(lane) * 128u;
+                // a staged box of 32 rows x 128 bytes; it is free once the store before has read it
+                if (p.c_tma_ok && ptx::elect_one()) ptx::tma_store_wait_read<0>();
+                __syncwarp();
+                const uint32_t row_addr = stage_base + static_cast<uint32_t>(lane) * 128u;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        ptx::st_shared_v4(row_addr + static_cast<uint32_t>((j ^ (lane & 7)) * 16), u[4 * j], u[4 * j + 1],
-                                          u[4 * j + 2], u[4 * j + 3]);
+                for (int j = 0; j < 8; ++j)
+                    ptx::st_shared_v4(row_addr + static_cast<uint32_t>((j ^ (lane & 7)) * 16), u[4 * j], u[4 * j + 1],
+                                      u[4 * j + 2], u[4 * j + 3]);
+                if (p.c_tma_ok) {
                     ptx::fence_proxy_async_smem();
                     __syncwarp();
                     if (ptx::elect_one()) {
@@ -762,20 +804,10 @@ gemm_e8m0_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
                         else ptx::tma_store_3d(&tmap_c, stage_base, n0, row0, 0);
                         ptx::tma_store_commit();
                     }
-                } else if (row0 + lane < p.M) {
-                    uint8_t* dst = static_cast<uint8_t*>(p.C) + (static_cast<long long>(row0 + lane) * p.ldc + n0) * OB;
-#pragma unroll
-                    for (int j = 0; j < CW; ++j) {
-                        if (n0 + j < p.N) {
-                            if constexpr (OUT == OUT_F32) {
-                                float* f = reinterpret_cast<float*>(dst) + j;
-                                *f = p.accumulate ? *f + __uint_as_float(u[j]) : __uint_as_float(u[j]);
-                            } else {
-                                reinterpret_cast<uint16_t*>(dst)[j] =
-                                    static_cast<uint16_t>((j & 1) ? (u[j >> 1] >> 16) : (u[j >> 1] & 0xffffu));
-                            }
-                        }
-                    }
+                } else {
+                    __syncwarp();
+                    store_box_rows<OUT>(p, stage_base, row0, n0, lane);
+                    __syncwarp();
                 }
             }
         }
