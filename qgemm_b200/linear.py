@@ -17,13 +17,37 @@ c)`` (src/mix_gemm/hip_mix_gemm_kernel.cpp:508-516) is the forward product alone
 from __future__ import annotations
 
 from contextlib import nullcontext
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 
 import torch
 
-from . import ERR_INVALID_ARG, ERR_UNSUPPORTED, QgemmError, _matrix, _quantize_block, fp8_block_mm_e8m0, requantize_block
+from . import (BLOCK, ERR_INVALID_ARG, ERR_UNSUPPORTED, QgemmError, _dtype_code, _launch, _matrix, _quantize_block,
+               _scale_block_rows)
 
 _TYPES = (torch.bfloat16, torch.float16, torch.float32)
+_E4M3, _E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+
+
+class _Form:
+    """Where a row-form [rows, cols] matrix lies in a buffer of bytes: codes at ``codes`` with leading dimension ``ld``, scales
+    at ``scale``; ``end`` is where the next may start. A layer call keeps all its quantised matrices in one or two buffers:
+    for short calls making the tensors costs more than the GPU takes for them."""
+    __slots__ = ("rows", "cols", "block_rows", "codes", "ld", "scale", "end")
+
+    def __init__(self, start: int, rows: int, cols: int, square: bool = False):
+        self.rows, self.cols, self.block_rows = rows, cols, BLOCK if square else 1
+        self.codes, self.ld = start, (cols + 15) & -16
+        self.scale = (start + rows * self.ld + 127) & -128
+        self.end = (self.scale + self._scales() + 127) & -128
+
+    def _scales(self) -> int:
+        return -(-self.cols // BLOCK) * -(-self.rows // self.block_rows)
+
+    def tensors(self, buffer):
+        """(codes, scales) as tensors that share the buffer's memory."""
+        q = buffer[self.codes:self.codes + self.rows * self.ld].view(_E4M3).view(self.rows, self.ld)[:, :self.cols]
+        s = buffer[self.scale:self.scale + self._scales()].view(_E8M0)
+        return q, s.view(-(-self.cols // BLOCK), -(-self.rows // self.block_rows))
 
 
 @dataclass
@@ -45,16 +69,22 @@ class PackedWeight:
 
 @dataclass
 class LinearSaved:
-    """What :func:`fp8_linear_forward` keeps for :func:`fp8_linear_backward`. ``x_codes`` / ``x_scale`` are the 8-bit
-    checkpoint of the layer's input, [tokens, in] (:func:`qgemm_b200.dequantize_block` restores it)."""
-    x_codes: torch.Tensor | None
-    x_scale: torch.Tensor | None
-    weight_codes_t: torch.Tensor | None
-    weight_scale_t: torch.Tensor | None
+    """What :func:`fp8_linear_forward` keeps for :func:`fp8_linear_backward`. :attr:`x` is the 8-bit checkpoint of the layer's
+    input, ``(codes, scales)`` of [tokens, in] (:func:`qgemm_b200.dequantize_block` restores it); None if no gradient of the
+    weight was asked for."""
+    buffer: torch.Tensor | None  # x's codes, and the transposed weight's unless that is a packed one's
+    x_form: _Form | None
+    weight_form: _Form | None
+    weight_t: tuple | None  # (codes, scales) of a packed weight's transpose
     x_shape: tuple
     x_dtype: torch.dtype
     weight_dtype: torch.dtype | None
     out_features: int
+    device: torch.device = field(default=None)
+
+    @property
+    def x(self):
+        return None if self.x_form is None else self.x_form.tensors(self.buffer)
 
 
 def pack_weight(weight, backward: bool = False) -> PackedWeight:
@@ -64,11 +94,8 @@ def pack_weight(weight, backward: bool = False) -> PackedWeight:
         raise QgemmError(ERR_INVALID_ARG, "a weight is [out, in]")
     if weight.dtype not in _TYPES:
         raise QgemmError(ERR_UNSUPPORTED, f"a weight of dtype {weight.dtype}")
-    return PackedWeight(*_quantized(_rows(weight.detach()), True, True, backward))
-
-
-def _quantized(t, square: bool, row: bool, column: bool):
-    return _quantize_block(t, *_matrix("matrix", t), square, row, column)
+    w = _rows(weight.detach())
+    return PackedWeight(*_quantize_block(w, *_matrix("weight", w), True, True, backward))
 
 
 def _rows(t):
@@ -77,6 +104,13 @@ def _rows(t):
         return t
     # an empty matrix counts as contiguous whatever its strides
     return t.contiguous() if t.numel() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+def _tokens(shape) -> int:
+    tokens = 1
+    for d in shape[:-1]:
+        tokens *= d
+    return tokens
 
 
 def _flat(x, features: int, what: str):
@@ -93,11 +127,28 @@ def _flat(x, features: int, what: str):
     return _rows(x)
 
 
-def _tokens(shape) -> int:
-    tokens = 1
-    for d in shape[:-1]:
-        tokens *= d
-    return tokens
+def _quantize(device, t, base: int, row: _Form | None, column: _Form | None, square: bool = False) -> None:
+    """Quantises the matrix t into the forms of the buffer at address ``base``."""
+    rows, cols, ld = _matrix("matrix", t)
+    r = (base + row.codes, row.ld, base + row.scale) if row is not None else (None, 0, None)
+    c = (base + column.codes, column.ld, base + column.scale) if column is not None else (None, 0, None)
+    _launch("qgemm_quantize_block", device, _dtype_code(t), t.data_ptr(), ld, rows, cols, BLOCK if square else 1, *r, *c)
+
+
+def _product(device, a, b, c, m: int, n: int, k: int, accumulate: bool = False) -> None:
+    """c = a b^T; a and b: (address of codes, leading dimension, address of scales, rows a scale covers)."""
+    _, _, ldc = _matrix("c", c)
+    _launch("qgemm_fp8_block_e8m0_gemm", device, _dtype_code(c), a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3],
+            1 if accumulate else 0, c.data_ptr(), ldc, m, n, k)
+
+
+def _at(form: _Form, base: int):
+    return base + form.codes, form.ld, base + form.scale, form.block_rows
+
+
+def _of(codes, scale):
+    rows, cols, ld = _matrix("codes", codes)
+    return codes.data_ptr(), ld, scale.data_ptr(), _scale_block_rows("scale", scale, rows, cols, codes.device)
 
 
 def fp8_linear_forward(x, weight, need_dx: bool = True, need_dw: bool = True, out_dtype=None):
@@ -106,24 +157,53 @@ def fp8_linear_forward(x, weight, need_dx: bool = True, need_dw: bool = True, ou
     packed = isinstance(weight, PackedWeight)
     if not packed and (weight.dim() != 2 or weight.dtype not in _TYPES):
         raise QgemmError(ERR_INVALID_ARG, "a weight is a bf16, fp16 or fp32 matrix [out, in], or a PackedWeight")
-    if weight.device != x.device:
+    device = x.device
+    if weight.device != device:
         raise QgemmError(ERR_INVALID_ARG, "x and the weight are on different devices")
     out_features, in_features = weight.shape
     x2 = _flat(x, in_features, "x")
+    tokens = x2.shape[0]
     if packed:
         if need_dw:
             raise QgemmError(ERR_INVALID_ARG, "a PackedWeight has no gradient: need_dw=False")
         if need_dx and weight.codes_t is None:
             raise QgemmError(ERR_INVALID_ARG, "gradients with respect to x need pack_weight(..., backward=True)")
-        w, ws, wt, wts = weight.codes, weight.scale, weight.codes_t, weight.scale_t
+    # kept for the backward pass: x's codes, the weight's transpose; behind them what only this call needs
+    at = 0
+    x_form = w_form = wt_form = None
+    if need_dw:
+        x_form = _Form(0, tokens, in_features)
+        at = x_form.end
+    if need_dx and not packed:
+        wt_form = _Form(at, in_features, out_features, True)
+        at = wt_form.end
+    kept = at
+    if x_form is None:
+        x_form = _Form(at, tokens, in_features)
+        at = x_form.end
+    if not packed:
+        w_form = _Form(at, out_features, in_features, True)
+        at = w_form.end
+    buffer = torch.empty(kept, dtype=torch.uint8, device=device) if kept else None
+    scratch = torch.empty(at - kept, dtype=torch.uint8, device=device) if at > kept else None
+    base = buffer.data_ptr() if kept else 0
+    scratch_base = scratch.data_ptr() - kept if at > kept else 0
+    x_base = base if need_dw else scratch_base
+    if packed:
+        w_at = _of(weight.codes, weight.scale)
     else:
-        w, ws, *turned = _quantized(_rows(weight.detach()), True, True, need_dx)
-        wt, wts = turned if turned else (None, None)
-    xq, xs = _quantized(x2, False, True, False)
-    y = torch.empty((x2.shape[0], out_features), dtype=out_dtype or x.dtype, device=x.device)
-    fp8_block_mm_e8m0(xq, w, xs, ws, y)
-    saved = LinearSaved(xq if need_dw else None, xs if need_dw else None, wt if need_dx else None, wts if need_dx else None,
-                        tuple(x.shape), x.dtype, None if packed else weight.dtype, out_features)
+        w = _rows(weight.detach() if weight.requires_grad else weight)
+        rows, cols, ld = _matrix("weight", w)
+        turned = (base + wt_form.codes, wt_form.ld, base + wt_form.scale) if wt_form is not None else (None, 0, None)
+        _launch("qgemm_quantize_block", device, _dtype_code(w), w.data_ptr(), ld, rows, cols, BLOCK,
+                scratch_base + w_form.codes, w_form.ld, scratch_base + w_form.scale, *turned)
+        w_at = _at(w_form, scratch_base)
+    _quantize(device, x2, x_base, x_form, None)
+    y = torch.empty((tokens, out_features), dtype=out_dtype or x.dtype, device=device)
+    _product(device, _at(x_form, x_base), w_at, y, tokens, out_features, in_features)
+    saved = LinearSaved(buffer, x_form if need_dw else None, wt_form,
+                        (weight.codes_t, weight.scale_t) if packed and need_dx else None, tuple(x.shape), x.dtype,
+                        None if packed else weight.dtype, out_features, device)
     return (y if x.dim() == 2 else y.view(*x.shape[:-1], out_features)), saved
 
 
@@ -131,32 +211,54 @@ def fp8_linear_backward(dy, saved: LinearSaved, dw=None, accumulate: bool = Fals
     """``(dx, dw)`` from dy [..., out] and what the forward call saved; None for a gradient it saved nothing for. ``dw``: a
     matrix [out, in] to write into instead of a new one, or with ``accumulate`` (fp32) to add to, as over the micro-batches
     of one step."""
-    dy2 = _flat(dy, saved.out_features, "dy")
-    in_features = saved.x_shape[-1]
-    need_dx, need_dw = saved.weight_codes_t is not None, saved.x_codes is not None
+    out_features, in_features = saved.out_features, saved.x_shape[-1]
+    dy2 = _flat(dy, out_features, "dy")
+    device = saved.device
+    need_dx, need_dw = saved.weight_form is not None or saved.weight_t is not None, saved.x_form is not None
     tokens = _tokens(saved.x_shape)
     if dy2.shape[0] != tokens:
         raise QgemmError(ERR_INVALID_ARG, f"dy has {dy2.shape[0]} rows, x had {tokens}")
-    kept = saved.x_codes if need_dw else saved.weight_codes_t
-    if kept is not None and kept.device != dy.device:
+    if dy.device != device:
         raise QgemmError(ERR_INVALID_ARG, "dy is on another device than the layer")
     if accumulate and dw is None:
         raise QgemmError(ERR_INVALID_ARG, "accumulate adds to a given dw")
-    if dw is not None and not need_dw:
-        raise QgemmError(ERR_INVALID_ARG, "the forward call saved nothing for dw")
+    if dw is not None:
+        if not need_dw:
+            raise QgemmError(ERR_INVALID_ARG, "the forward call saved nothing for dw")
+        if dw.dim() != 2 or tuple(dw.shape) != (out_features, in_features) or dw.device != device:
+            raise QgemmError(ERR_INVALID_ARG, f"dw is [{out_features}, {in_features}] on the layer's device")
+        _matrix("dw", dw)
+        if accumulate and dw.dtype != torch.float32:
+            raise QgemmError(ERR_UNSUPPORTED, "accumulate needs a fp32 dw")
     if not need_dx and not need_dw:
         return None, None
-    forms = _quantized(dy2, False, need_dx, need_dw)
+    at = 0
+    along = across = x_across = None
+    if need_dx:
+        along = _Form(at, tokens, out_features)
+        at = along.end
+    if need_dw:
+        across = _Form(at, out_features, tokens)
+        x_across = _Form(across.end, in_features, tokens)
+        at = x_across.end
+    scratch = torch.empty(at, dtype=torch.uint8, device=device)
+    base = scratch.data_ptr()
+    kept = saved.buffer.data_ptr() if saved.buffer is not None else 0
+    _quantize(device, dy2, base, along, across)
     dx = None
     if need_dx:
-        dx = torch.empty((tokens, in_features), dtype=saved.x_dtype, device=dy.device)
-        fp8_block_mm_e8m0(forms[0], saved.weight_codes_t, forms[1], saved.weight_scale_t, dx)
-        dx = dx.view(saved.x_shape)
+        dx = torch.empty((tokens, in_features), dtype=saved.x_dtype, device=device)
+        w_at = _at(saved.weight_form, kept) if saved.weight_form is not None else _of(*saved.weight_t)
+        _product(device, _at(along, base), w_at, dx, tokens, in_features, out_features)
+        if len(saved.x_shape) != 2:
+            dx = dx.view(saved.x_shape)
     if need_dw:
-        xt, xts = requantize_block(saved.x_codes, saved.x_scale)
+        f = saved.x_form
+        _launch("qgemm_requantize_block", device, kept + f.codes, f.ld, kept + f.scale, tokens, in_features,
+                base + x_across.codes, x_across.ld, base + x_across.scale)
         if dw is None:
-            dw = torch.empty((saved.out_features, in_features), dtype=saved.weight_dtype, device=dy.device)
-        fp8_block_mm_e8m0(forms[-2], xt, forms[-1], xts, dw, accumulate=accumulate)
+            dw = torch.empty((out_features, in_features), dtype=saved.weight_dtype, device=device)
+        _product(device, _at(across, base), _at(x_across, base), dw, out_features, in_features, tokens, accumulate)
     return dx, dw
 
 
@@ -174,8 +276,8 @@ class _Fp8Linear(torch.autograd.Function):
     def forward(ctx, x, weight, packed, out_dtype):
         need_dx, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
         y, saved = fp8_linear_forward(x, weight if packed is None else packed, need_dx, need_dw, out_dtype)
-        ctx.save_for_backward(saved.x_codes, saved.x_scale, saved.weight_codes_t, saved.weight_scale_t)
-        saved.x_codes = saved.x_scale = saved.weight_codes_t = saved.weight_scale_t = None
+        ctx.save_for_backward(saved.buffer, *(saved.weight_t or ()))
+        saved.buffer = saved.weight_t = None
         ctx.rest = saved
         return y
 
@@ -183,7 +285,9 @@ class _Fp8Linear(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         r = ctx.rest
-        saved = LinearSaved(*ctx.saved_tensors, r.x_shape, r.x_dtype, r.weight_dtype, r.out_features)
+        buffer, *weight_t = ctx.saved_tensors
+        saved = LinearSaved(buffer, r.x_form, r.weight_form, tuple(weight_t) or None, r.x_shape, r.x_dtype, r.weight_dtype,
+                            r.out_features, r.device)
         dx, dw = fp8_linear_backward(dy, saved)
         return dx, dw, None, None
 

@@ -140,8 +140,9 @@ def test_checkpoint_restores_the_activation(qlib, dev):
     from qgemm_b200.linear import fp8_linear_forward
     x, w = _data(90, 512, torch.bfloat16, dev, 1), _data(64, 512, torch.bfloat16, dev, 2)
     _, saved = fp8_linear_forward(x, w)
-    assert saved.x_codes.element_size() == 1
-    back = qlib.dequantize_block(saved.x_codes, saved.x_scale, torch.bfloat16)
+    codes, scale = saved.x
+    assert codes.element_size() == 1 and codes.shape == x.shape
+    back = qlib.dequantize_block(codes, scale, torch.bfloat16)
     assert torch.equal(back.cpu(), _q(x).to(torch.float32).to(torch.bfloat16))
 
 
