@@ -237,7 +237,7 @@ int qgemm_plan_query_ex(int in_dtype, int out_dtype, int b_layout, size_t M, siz
 /*
  * Synchronises the current device and copies its four status words to out4:
  * [0] error code (0 = none, 1 = a bounded wait ran out), [1] CTA, [2] role (1 producer, 2 MMA,
- * 3 epilogue), [3] position. Returns QGEMM_ERR_DEVICE_TIMEOUT if [0] != 0. Clears the words.
+ * 3 epilogue, 4 scales), [3] position. Returns QGEMM_ERR_DEVICE_TIMEOUT if [0] != 0. Clears the words.
  * The words of qgemm_mix_gemm_splitk_static (which keeps its own, inside the loaded module) are read and
  * cleared as well and reported when the ordinary ones are clean. Allocates nothing: on a device where no
  * GEMM has run yet there is nothing to read.

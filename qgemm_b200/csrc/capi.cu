@@ -974,7 +974,7 @@ double estimate_e8m0(const E8m0Plan& pl, size_t M, size_t N, size_t K, int sms) 
         }
         const double rounds = std::ceil(tiles / (sms / 2));
         if (pl.tile_n == 128) return 4.6 + std::max(rounds * (kb * 0.235 + 1.3), hbm);
-        return 6.5 + std::max(rounds * (kb * 0.345 + 1.0), hbm);
+        return 6.0 + std::max(rounds * (kb * 0.345 + 0.6), hbm);
     }
     // clusters of four and eight do not fill every SM's two places
     const double places = 2.0 * sms * (pl.slices == 8 ? 0.87 : (pl.slices == 4 ? 0.95 : 1.0));
@@ -1097,6 +1097,7 @@ int e8m0_launch(const E8m0Plan& plan, const void* A, size_t lda, const void* B, 
     const size_t out_bytes = (p.out == OUT_F32) ? 4 : 2;
     const uintptr_t c_addr = reinterpret_cast<uintptr_t>(p.C);
     p.kb_total = (p.K + 127) / 128;
+    p.test_skip_kb = take_test_skip_kb();
     p.c_vec_ok = c_addr % (4 * out_bytes) == 0 && p.ldc % 4 == 0;
     p.m_tiles = (p.M + plan.tile_m - 1) / plan.tile_m;
     p.n_tiles = (p.N + plan.tile_n - 1) / plan.tile_n;

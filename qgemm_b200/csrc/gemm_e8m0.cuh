@@ -37,12 +37,19 @@ struct E8m0Params {
     int out;               // OUT_F32 / OUT_BF16 / OUT_F16
     int accumulate;        // fp32 C: add to what it holds
     int c_tma_ok, c_vec_ok;
+    int test_skip_kb;  // failure-detection test hook: the producers leave out this K block (-1 = none)
     int* status;
 };
 
 constexpr int kE8Cols = 4;       // chunks of scales in tensor memory
 constexpr int kE8Threads = 320;  // producer, MMA issuer, four epilogue warps, four scale warps (6 .. 9)
 enum : int { ROLE_SCALES = 4 };
+
+// wait_bounded by a whole warp, with one answer: what follows is executed by all its lanes or by none.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int role,
+                                          int where, uint32_t peer_abort = 0) {
+    return __all_sync(0xffffffffu, wait_bounded(bar, parity, abort_flag, status, role, where, peer_abort));
+}
 
 // One operand's scales on their way from global to shared memory.
 struct ScaleSource {
@@ -160,7 +167,7 @@ struct ScaleFeeder {
                 if (g < UNITS) put_scales(area + g * 512, buf[i], src, put.row0, put.kb, min(4, kb1 - put.kb), lane);
                 fetch(buf[i], rows);
                 asm volatile("bar.sync 1, 128;" ::: "memory");
-                ok = ok && __all_sync(0xffffffffu, free(i, parity, put.kb));
+                ok = ok && free(i, parity, put.kb);
                 if (ok) {
                     ptx::tc_fence_after();
                     uint4 v[UNITS];
@@ -325,6 +332,7 @@ gemm_e8m0_small_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
     const int kb1 = static_cast<int>(static_cast<long long>(rank + 1) * p.kb_total / S);
 
     auto load_block = [&](int kb, uint32_t stage) {
+        if (kb == p.test_skip_kb) return;
         const uint32_t full = bar_full + stage * 8;
         ptx::mbar_arrive_expect_tx(full, L::kBStage + L::kAStage);
         ptx::tma_load_2d(smem_b + stage * L::kBStage, &tmap_b, full, kb * 128, n0);
@@ -450,7 +458,7 @@ gemm_e8m0_small_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
     } else if (warp >= 6) {
         // ------------------------------------------------------------ scales
         auto free = [&](int col, uint32_t parity, int kb) {
-            const bool ok = wait_bounded(bar_sdone + col * 8, parity, abort_flag, p.status, ROLE_SCALES, kb);
+            const bool ok = warp_wait(bar_sdone + col * 8, parity, abort_flag, p.status, ROLE_SCALES, kb);
             if (!ok) raise_peers();
             return ok;
         };
@@ -459,7 +467,7 @@ gemm_e8m0_small_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
     } else {
         // ------------------------------------------------------------ accumulator -> own shared memory, a token a row
         const int quad = warp & 3;
-        if (wait_bounded(bar_tfull, 0u, abort_flag, p.status, ROLE_EPILOGUE, tile)) {
+        if (warp_wait(bar_tfull, 0u, abort_flag, p.status, ROLE_EPILOGUE, tile)) {
             ptx::tc_fence_after();
             // the ring is idle: every load has landed and every MMA that read it has completed
             float* col = reinterpret_cast<float*>(smem) + quad * 32 + lane;
@@ -652,10 +660,12 @@ gemm_e8m0_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
                         ok = false;
                         break;
                     }
-                    if (rank == 0) ptx::mbar_arrive_expect_tx(bar_full + stage * 8, 2 * (L::kAStage + L::kBStage));
-                    const uint32_t leader_full = ptx::mapa_shared(bar_full + stage * 8, 0);
-                    ptx::tma_load_2d_pair(smem_a + stage * L::kAStage, &tmap_a, leader_full, kb * 128, row_a);
-                    ptx::tma_load_2d_pair(smem_b + stage * L::kBStage, &tmap_b, leader_full, kb * 128, row_b);
+                    if (kb != p.test_skip_kb) {
+                        if (rank == 0) ptx::mbar_arrive_expect_tx(bar_full + stage * 8, 2 * (L::kAStage + L::kBStage));
+                        const uint32_t leader_full = ptx::mapa_shared(bar_full + stage * 8, 0);
+                        ptx::tma_load_2d_pair(smem_a + stage * L::kAStage, &tmap_a, leader_full, kb * 128, row_a);
+                        ptx::tma_load_2d_pair(smem_b + stage * L::kBStage, &tmap_b, leader_full, kb * 128, row_b);
+                    }
                     if (++stage == STAGES) {
                         stage = 0;
                         phase ^= 1u;
@@ -733,7 +743,7 @@ gemm_e8m0_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
         feeder.kb1 = p.kb_total;
         feeder.start(scale_rows);
         auto free = [&](int col, uint32_t parity, int kb) {
-            return wait_bounded(bar_sdone + col * 8, parity, abort_flag, p.status, ROLE_SCALES, kb, peer_abort);
+            return warp_wait(bar_sdone + col * 8, parity, abort_flag, p.status, ROLE_SCALES, kb, peer_abort);
         };
         auto ready = [&](int col) { ptx::mbar_arrive_remote(ptx::mapa_shared(bar_sfull + col * 8, 0)); };
         feeder.run(scale_rows, smem_s, tmem_base + L::kScaleCol, warp & 3, free, ready);
@@ -746,7 +756,7 @@ gemm_e8m0_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
             int m_blk, n_blk;
             e8_decode(w, p, m_blk, n_blk);
             const uint32_t acc = it & 1u;
-            if (!wait_bounded(bar_tfull + acc * 8, (it >> 1) & 1u, abort_flag, p.status, ROLE_EPILOGUE, w, peer_abort)) break;
+            if (!warp_wait(bar_tfull + acc * 8, (it >> 1) & 1u, abort_flag, p.status, ROLE_EPILOGUE, w, peer_abort)) break;
             ptx::tc_fence_after();
             const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * L::kAccStep;
             const int row0 = (m_blk * 2 + static_cast<int>(rank)) * 128 + quad * 32;
@@ -769,7 +779,7 @@ gemm_e8m0_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
                 if (b == kShared - 1) {
                     ptx::tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) ptx::mbar_arrive_cluster(ptx::mapa_shared(bar_tfree + (kOverlap ? 0 : acc * 8), 0));
+                    if (lane == 0) ptx::mbar_arrive_remote(ptx::mapa_shared(bar_tfree + (kOverlap ? 0 : acc * 8), 0));
                 }
                 if (!live) continue;
                 uint32_t u[32];
@@ -938,11 +948,13 @@ gemm_e8m0_pair_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __
                     raise_peers();
                     break;
                 }
-                if (rank == 0) ptx::mbar_arrive_expect_tx(bar_full + stage * 8, 2 * (L::kAStage + L::kBStage));
-                const uint32_t leader_full = ptx::mapa_shared(bar_full + stage * 8, leader);
-                ptx::tma_load_2d_pair(smem_a + stage * L::kAStage, &tmap_a, leader_full, kb * 128, m0);
-                ptx::tma_load_2d_pair(smem_b + stage * L::kBStage, &tmap_b, leader_full, kb * 128,
-                                      n0 + static_cast<int>(rank) * 64);
+                if (kb != p.test_skip_kb) {
+                    if (rank == 0) ptx::mbar_arrive_expect_tx(bar_full + stage * 8, 2 * (L::kAStage + L::kBStage));
+                    const uint32_t leader_full = ptx::mapa_shared(bar_full + stage * 8, leader);
+                    ptx::tma_load_2d_pair(smem_a + stage * L::kAStage, &tmap_a, leader_full, kb * 128, m0);
+                    ptx::tma_load_2d_pair(smem_b + stage * L::kBStage, &tmap_b, leader_full, kb * 128,
+                                          n0 + static_cast<int>(rank) * 64);
+                }
                 if (++stage == STAGES) {
                     stage = 0;
                     phase ^= 1u;
@@ -994,7 +1006,7 @@ gemm_e8m0_pair_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __
     } else if (warp >= 6) {
         // ------------------------------------------------------------ scales (every CTA)
         auto free = [&](int col, uint32_t parity, int kb) {
-            const bool ok = wait_bounded(bar_sdone + col * 8, parity, abort_flag, p.status, ROLE_SCALES, kb);
+            const bool ok = warp_wait(bar_sdone + col * 8, parity, abort_flag, p.status, ROLE_SCALES, kb);
             if (!ok) raise_peers();
             return ok;
         };
@@ -1004,7 +1016,7 @@ gemm_e8m0_pair_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __
     } else {
         // ------------------------------------------------------------ accumulator -> own shared memory
         const int quad = warp & 3;
-        if (wait_bounded(bar_tfull, 0u, abort_flag, p.status, ROLE_EPILOGUE, m_blk)) {
+        if (warp_wait(bar_tfull, 0u, abort_flag, p.status, ROLE_EPILOGUE, m_blk)) {
             ptx::tc_fence_after();
             // the ring is idle: every load has landed and every MMA that read it, in either CTA, has completed
             if (m0 + quad * 32 < p.M) {  // rows that exist

@@ -341,3 +341,155 @@ def test_product_empty(qlib, dev):
         assert bool((c == 3).all())
         qlib.fp8_block_mm_e8m0(a, b, sa, sb, c)
         assert bool((c == 0).all())
+
+
+# ------------------------------------------------------------------------------------------------ far, odd and refused calls
+def test_offsets_past_32_bits(qlib, dev):
+    """More than 2^32 elements: the last rows and columns of every result, on values made for them."""
+    rows, cols = 66100, 65536
+    x = torch.zeros(rows, cols, dtype=torch.bfloat16, device=dev)
+    tail = _data(300, 700, torch.bfloat16, dev, 1)
+    x[-300:, -700:] = tail
+    q, s, qt, st = qlib.quantize_block(x, form="both")
+    first, lead = rows - 300, cols - 700
+    start_c, start_r = lead // 128 * 128, first // 128 * 128  # whole blocks, the zeros in front included
+    q_ref, s_ref = quantize(x[first:, start_c:])
+    assert torch.equal(bytes_of(q[first:, start_c:]), q_ref)
+    assert torch.equal(bytes_of(s)[start_c // 128:, first:], s_ref)
+    qt_ref, st_ref = quantize(x[start_r:, lead:].t())
+    assert torch.equal(bytes_of(qt[lead:, start_r:]), qt_ref)
+    assert torch.equal(bytes_of(st)[start_r // 128:, lead:], st_ref)
+    assert int(q.view(torch.uint8)[:first].count_nonzero()) == 0
+    del x, qt, st
+    back = torch.empty(rows, cols, dtype=torch.bfloat16, device=dev)
+    qlib.dequantize_block(q, s, out=back)
+    assert torch.equal(back[first:, start_c:].cpu(), values(q_ref, s_ref).to(torch.bfloat16))
+    del back
+    ct, cts = qlib.requantize_block(q, s)
+    full = values(q[start_r:, start_c:], s[start_c // 128:, start_r:].contiguous())[:, lead - start_c:]
+    ct_ref, cts_ref = quantize(full.t())
+    assert torch.equal(bytes_of(ct[lead:, start_r:]), ct_ref)
+    assert torch.equal(bytes_of(cts)[start_r // 128:, lead:], cts_ref)
+    del ct, cts
+    # a product whose A has more than 2^32 codes, and one whose C has more than 2^32 elements
+    w = _data(24, cols, torch.bfloat16, dev, 2)
+    b, sb = qlib.quantize_block(w)
+    c = torch.empty(rows, 24, device=dev)
+    qlib.fp8_block_mm_e8m0(q, b, s, sb, c)
+    av = values(q[first:, start_c:], s[start_c // 128:, first:].contiguous())
+    bv = values(b[:, start_c:], sb[start_c // 128:].contiguous())
+    _assert_close(c[first:], (av @ bv.t()).to(dev), (av.abs() @ bv.abs().t()).to(dev), cols, torch.float32)
+    assert int(c[:first].count_nonzero()) == 0
+    del q, s, c
+    (a, sa), (b, sb) = (qlib.quantize_block(_data(n, 64, torch.bfloat16, dev, n, 1.0)) for n in (66000, 65600))
+    c = torch.empty(66000, 65600, dtype=torch.bfloat16, device=dev)
+    qlib.fp8_block_mm_e8m0(a, b, sa, sb, c)
+    av, bv = values(a[-300:], sa[:, -300:].contiguous()), values(b, sb)
+    _assert_close(c[-300:], (av @ bv.t()).to(dev), (av.abs() @ bv.abs().t()).to(dev), 64, torch.bfloat16)
+
+
+@pytest.mark.parametrize("tile_m,tile_n,slices", [(16, 128, 1), (32, 128, 8), (64, 128, 4), (256, 256, 1), (256, 128, 1), (256, 128, 2)])
+def test_a_wait_that_runs_out_is_reported(qlib, dev, monkeypatch, tile_m, tile_n, slices):
+    """The host leaves out the loads of one K block (a hook of the library): the issuer's wait for it ends after about a
+    second, every role and every CTA of the cluster leaves, the status says where, and the next call is right."""
+    M, N, K = (16, 128, 2048) if tile_m != 256 else (256, tile_n, 2048)
+    a, sa, b, sb = _operands(qlib, dev, M, N, K, False, True, 5)
+    ref, mags = _product(a, sa, b, sb)
+    c = torch.empty(M, N, device=dev)
+    monkeypatch.setenv("QGEMM_E8M0_TILE_M", str(tile_m))
+    monkeypatch.setenv("QGEMM_E8M0_TILE_N", str(tile_n))
+    monkeypatch.setenv("QGEMM_E8M0_SLICES", str(slices))
+    qlib.lib().qgemm_reload_env()
+    try:
+        assert qlib.device_status()[0] == qlib.OK
+        qlib.lib().qgemm_test_arm_skip_load(1)
+        qlib.fp8_block_mm_e8m0(a, b, sa, sb, c)
+        rc, st = qlib.device_status()
+        assert rc == qlib.ERR_DEVICE_TIMEOUT
+        # the MMA issuer, waiting for K block 1, or the producer, which within the same microseconds and for as long starts
+        # to wait for that block's slot to come free
+        assert st[0] == 1 and ((st[2] == 2 and st[3] == 1) or (st[2] == 1 and st[3] > 1)), st
+        assert qlib.device_status()[0] == qlib.OK
+        qlib.fp8_block_mm_e8m0(a, b, sa, sb, c)
+        assert qlib.device_status()[0] == qlib.OK
+    finally:
+        monkeypatch.undo()
+        qlib.lib().qgemm_reload_env()
+    _assert_close(c, ref, mags, K, torch.float32)
+
+
+def test_captured_on_a_side_stream_with_forms_not_used_before(qlib, dev):
+    """A graph of quantiser and products of several sizes replays on new values, twice with other work between."""
+    sizes = [(3, 1000, 384), (40, 264, 2176), (200, 520, 1152), (700, 800, 300), (1500, 1300, 256)]
+    xs = [_data(m, k, torch.bfloat16, dev, m, 1.0) for m, _, k in sizes]
+    ws = [_data(n, k, torch.float32, dev, n, 1.0) for _, n, k in sizes]
+
+    def run():
+        outs = []
+        for x, w in zip(xs, ws):
+            a, sa = qlib.quantize_block(x)
+            b, sb = qlib.quantize_block(w, square=True)
+            c = torch.empty(x.shape[0], w.shape[0], device=dev)
+            qlib.fp8_block_mm_e8m0(a, b, sa, sb, c)
+            t, st = qlib.requantize_block(a, sa)
+            outs += [c, qlib.dequantize_block(a, sa), t.view(torch.uint8), st.view(torch.uint8)]
+        return outs
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        held = run()
+    for seed in (1, 2):
+        for t in xs + ws:
+            t.copy_(_data(*t.shape, t.dtype, dev, seed + t.shape[0], 1.0))
+        graph.replay()
+        want = run()
+        torch.cuda.synchronize()
+        for h, w in zip(held, want):
+            assert torch.equal(h, w)
+
+
+def test_single_rows_columns_and_odd_strides(qlib, dev):
+    wide = _data(70, 400, torch.bfloat16, dev, 3, 1.0)
+    for x in (wide[:, 17:18], wide[5:6], wide[::3], wide[::2, 8:264], wide[3:4, 9:10]):
+        _check_forms(qlib, x, False)
+        _check_forms(qlib, x, True)
+    for bad in (wide.t(), wide[:, ::2], wide[:, :1].t(), wide[:1].expand(70, 400), wide.view(70, 20, 20)):
+        with pytest.raises(qlib.QgemmError) as e:
+            qlib.quantize_block(bad)
+        assert e.value.status == qlib.ERR_INVALID_ARG
+
+
+def test_python_refusals(qlib, dev):
+    x = _data(40, 256, torch.bfloat16, dev, 1)
+    q, s, qt, st = qlib.quantize_block(x, form="both")
+    c = torch.zeros(40, 40, device=dev)
+    inv, uns, ali = qlib.ERR_INVALID_ARG, qlib.ERR_UNSUPPORTED, qlib.ERR_ALIGNMENT
+    odd = torch.zeros(40, 272, dtype=torch.uint8, device=dev).view(E4M3)
+    calls = [
+        (inv, lambda: qlib.quantize_block(x, form="rows")),
+        (uns, lambda: qlib.quantize_block(x.double())),
+        (inv, lambda: qlib.quantize_block(x, out=(q, s, qt, st))),
+        (inv, lambda: qlib.quantize_block(x, out=(qt, st))),
+        (inv, lambda: qlib.quantize_block(x, out=(q, s.float()))),
+        (inv, lambda: qlib.quantize_block(x, square=True, out=(q, s))),
+        (inv, lambda: qlib.requantize_block(q.view(torch.uint8), s)),
+        (inv, lambda: qlib.requantize_block(q, s[:1])),
+        (uns, lambda: qlib.requantize_block(*qlib.quantize_block(x, square=True))),
+        (inv, lambda: qlib.dequantize_block(q, s, torch.bfloat16, out=c)),
+        (uns, lambda: qlib.dequantize_block(q, s, torch.int8)),
+        (inv, lambda: qlib.fp8_block_mm_e8m0(q, qt, s, st, c)),
+        (inv, lambda: qlib.fp8_block_mm_e8m0(q, q, s, s, c[:39])),
+        (inv, lambda: qlib.fp8_block_mm_e8m0(q, q, s, s.view(torch.uint8), c)),
+        (inv, lambda: qlib.fp8_block_mm_e8m0(q, q, s, s[:, ::2], c)),
+        (inv, lambda: qlib.fp8_block_mm_e8m0(q, q, s, s.cpu(), c)),
+        (inv, lambda: qlib.fp8_block_mm_e8m0(q, q, s, s, c[:1].expand(40, 40))),
+        (uns, lambda: qlib.fp8_block_mm_e8m0(q, q, s, s, c.bfloat16(), accumulate=True)),
+        (uns, lambda: qlib.fp8_block_mm_e8m0(q, q, s, s, c.to(torch.int32))),
+        (ali, lambda: qlib.fp8_block_mm_e8m0(odd[:, 8:264], q, s, s, c)),
+        (ali, lambda: qlib.fp8_block_mm_e8m0(odd.view(torch.uint8).flatten()[:40 * 264].view(E4M3).view(40, 264)[:, :256], q, s, s, c)),
+    ]
+    for status, call in calls:
+        with pytest.raises(qlib.QgemmError) as e:
+            call()
+        assert e.value.status == status
+    assert bool((c == 0).all())

@@ -251,3 +251,42 @@ def test_layer_refusals(qlib, dev):
         fp8_linear_backward(y, saved, dw=torch.zeros(32, 64, device=dev, dtype=torch.bfloat16), accumulate=True)
     with pytest.raises(qlib.QgemmError):
         fp8_linear_backward(y, saved, dw=torch.zeros(31, 64, device=dev))
+
+
+def test_broadcast_input_gets_the_sum_of_its_gradients(qlib, dev):
+    from qgemm_b200.linear import fp8_linear
+    base, w = _data(1, 256, torch.float32, dev, 1), _data(130, 256, torch.float32, dev, 2)
+    dy = _data(9, 130, torch.float32, dev, 3)
+    b = base.clone().requires_grad_(True)
+    fp8_linear(b.expand(9, 256), w).backward(dy)
+    full = base.expand(9, 256).clone().requires_grad_(True)
+    fp8_linear(full, w).backward(dy)
+    assert torch.equal(b.grad, full.grad.sum(0, keepdim=True))
+    # one weight in two layers of one graph
+    x, u = _data(20, 130, torch.float32, dev, 4, 0.5), _data(130, 130, torch.float32, dev, 5, 0.5).requires_grad_(True)
+    y = fp8_linear(x, u)
+    z = fp8_linear(y, u)
+    z.sum().backward()
+    first = y.detach().requires_grad_(True)
+    v = u.detach().clone().requires_grad_(True)
+    fp8_linear(first, v).sum().backward()
+    t = u.detach().clone().requires_grad_(True)
+    fp8_linear(x, t).backward(first.grad)
+    assert torch.equal(u.grad, v.grad + t.grad) or torch.equal(u.grad, t.grad + v.grad)
+
+
+def test_backward_twice_and_on_another_thread(qlib, dev):
+    import threading
+
+    from qgemm_b200.linear import fp8_linear
+    x, w = _data(33, 256, torch.bfloat16, dev, 1).requires_grad_(True), _data(140, 256, torch.bfloat16, dev, 2).requires_grad_(True)
+    dy = _data(33, 140, torch.bfloat16, dev, 3)
+    y = fp8_linear(x, w)
+    one = torch.autograd.grad(y, (x, w), dy, retain_graph=True)
+    two = torch.autograd.grad(y, (x, w), dy, retain_graph=True)
+    got = []
+    t = threading.Thread(target=lambda: got.extend(torch.autograd.grad(y, (x, w), dy)))
+    t.start()
+    t.join()
+    for a, b, c in zip(one, two, got):
+        assert torch.equal(a, b) and torch.equal(a, c)
