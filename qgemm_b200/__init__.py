@@ -395,9 +395,9 @@ def _new_form(rows: int, cols: int, square: bool, device):
     their scales."""
     torch = _torch()
     ld = -(-cols // 16) * 16
-    q = torch.empty((rows, ld), dtype=torch.float8_e4m3fn, device=device)
+    q = torch.empty_strided((rows, cols), (ld, 1), dtype=torch.float8_e4m3fn, device=device)
     s = torch.empty((-(-cols // BLOCK), -(-rows // BLOCK) if square else rows), dtype=torch.float8_e8m0fnu, device=device)
-    return (q if ld == cols else q[:, :cols]), ld, s
+    return q, ld, s
 
 
 def _given_form(out, rows: int, cols: int, square: bool, what: str, device):

@@ -12,8 +12,8 @@
 // of 32 lanes, repeated over the four lane quadrants. They come from global memory in the caller's plain layout ([K
 // block][row], or [K block][row / 128]) through four warps, one a quadrant: a warp a 128 rows loads words and turns them into
 // a row's four K blocks, and after an exchange through shared memory every warp stores all of them to its quadrant.
-// (Shared memory -> tensor memory with tcgen05.cp takes its place among the MMAs instead: at 4096 x 7168 x 7168 the product
-// took 156 us with it, 139 with the copies left out.)
+// (Through tcgen05.cp instead, from shared memory and in the issuing thread's own order, the issuer had two more waits, the
+// copies and two more commits for every chunk: 256 x 128 tiles took 21.9 us for 1024 x 2048 x 8192, with stores 19.4.)
 //
 // Barriers besides the ring's full / empty and the accumulators': sfull[c] (a chunk's scales are in columns c), sdone[c]
 // (the chunk's last MMA has completed: columns c are free). All waits are bounded as in gemm_sm100.cuh.
@@ -118,8 +118,9 @@ __device__ __forceinline__ void put_scales(uint32_t dst, const ScaleWords& c, co
 
 // The four scale warps, over the chunks of K blocks [kb0, kb1) of work items first, first + step, ... < last. Unit u = 0 ..
 // UNITS - 1 is 128 rows of an operand, loaded by scale warp u from row rows(work item). `start` sends the first loads on their
-// way (before the CTA-wide barrier); `run` needs tensor memory, and is executed by all four warps to the end whatever
-// happens, because they meet at a barrier of their own for every chunk: after a wait that ran out they only meet.
+// way; `run` needs tensor memory, and is executed by all four warps to the end whatever
+// happens, because they meet at a barrier of their own for every chunk: after a wait that ran out they only meet. (`start` may
+// come before the CTA-wide barrier of a kernel whose other warps wait there for memory too.)
 template <int UNITS>
 struct ScaleFeeder {
     ScaleSource src;
@@ -518,8 +519,10 @@ gemm_e8m0_small_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
 // CTA pairs on 256 x 256 tiles (tcgen05.mma.cta_group::2; the ring, the pair's barriers and the persistent tile loop as in
 // gemm_sm100_2cta.cuh). Each CTA's tensor memory has 512 columns: two 256-column accumulators would leave none for scales,
 // so the second accumulator starts at column 192 and the last 64 columns hold four chunks of scales. The accumulators
-// share columns 192..255: the epilogue drains those first and hands them over (`ovl`), and the next tile's MMAs run under
-// the rest of the drain. The first instruction of a tile waits only for a quarter of its predecessor's epilogue.
+// share columns 192..255: the epilogue drains those first and hands them over (`tfree`), and the next tile's MMAs run under
+// the rest of the drain. The first instruction of a tile waits only for a quarter of its predecessor's epilogue; the arrival
+// that tells the issuer is in its way, so it orders no more than it must (mbar_arrive_remote; as a cluster-scope release it
+// made 6144 x 7168 x 2048 take 91 us instead of 85).
 //
 // Scales: the leader's instruction multiplies each CTA's 128 rows by that CTA's A scales, and all 256 columns by the B
 // scales, which both CTAs hold in full; the scale warps of either CTA arrive on the leader's `sfull`.
