@@ -262,7 +262,7 @@ def fp8_linear_backward(dy, saved: LinearSaved, dw=None, accumulate: bool = Fals
     return dx, dw
 
 
-_STREAM = "qgemm_b200.linear stream"
+_DEFAULT_STREAM = "qgemm_b200.linear: made on the default stream"
 
 
 def _accumulators(*leaves):
@@ -295,10 +295,10 @@ class _Fp8Linear(torch.autograd.Function):
 def fp8_linear(x, weight, out_dtype=None):
     """y = x W^T in 8 bits with autograd: x [..., in] bf16 / fp16 / fp32, ``weight`` [out, in] a matrix that may require a
     gradient, or a :class:`PackedWeight` (serving; frozen layers). y has x's type unless ``out_dtype`` says otherwise.
-    Runs on the current stream of x's device. A CUDA graph is captured after one ordinary call on the device. A leaf that an
-    earlier layer call's graph, still alive, refers to is refused in a capture: its gradient node belongs to that call's
-    stream, and torch would leave the capture in the backward pass. Delete what keeps that graph alive, or capture
-    :func:`fp8_linear_forward` and :func:`fp8_linear_backward`, which use no autograd."""
+    Runs on the current stream of x's device. A CUDA graph is captured after one ordinary call on the device. A leaf that the
+    graph of an earlier layer call on the default stream, still alive, refers to is refused in a capture: its gradient node
+    belongs to that stream, and torch would leave the capture in the backward pass. Delete what keeps that graph alive, or
+    capture :func:`fp8_linear_forward` and :func:`fp8_linear_backward`, which use no autograd."""
     packed = weight if isinstance(weight, PackedWeight) else None
     w = None if packed is not None else weight
     if not torch.is_grad_enabled() or not (x.requires_grad or (w is not None and w.requires_grad)):
@@ -306,11 +306,13 @@ def fp8_linear(x, weight, out_dtype=None):
     if not x.is_cuda:
         raise QgemmError(ERR_INVALID_ARG, "x must be a CUDA tensor (there is no CPU path)")
     stream = torch.cuda.current_stream(x.device).cuda_stream
-    with nullcontext() if torch.cuda.current_device() == x.device.index else torch.cuda.device(x.device):
-        capturing = torch.cuda.is_current_stream_capturing()
-    if capturing and any(n.metadata.get(_STREAM, stream) != stream for n in _accumulators(x, w)):
-        raise QgemmError(ERR_UNSUPPORTED, "capturing a graph while an earlier graph of the same leaves is alive")
+    if stream != 0:  # the default stream is never captured, and no other's graph hinders a capture
+        with nullcontext() if torch.cuda.current_device() == x.device.index else torch.cuda.device(x.device):
+            capturing = torch.cuda.is_current_stream_capturing()
+        if capturing and any(n.metadata.get(_DEFAULT_STREAM) for n in _accumulators(x, w)):
+            raise QgemmError(ERR_UNSUPPORTED, "capturing a graph while an earlier graph of the same leaves is alive")
     y = _Fp8Linear.apply(x, w, packed, out_dtype)
-    for node in _accumulators(x, w):  # alive as long as a graph refers to the leaf, and its marks with it
-        node.metadata.setdefault(_STREAM, stream)
+    if stream == 0:
+        for node in _accumulators(x, w):  # alive as long as a graph refers to the leaf, and its mark with it
+            node.metadata[_DEFAULT_STREAM] = True
     return y

@@ -332,6 +332,23 @@ def test_product_nan_blocks_reach_their_rows_only(qlib, dev):
     assert torch.equal(torch.isnan(c), bad)
 
 
+@pytest.mark.parametrize("M,N,K", [(5, 300, 1000), (333, 259, 700), (1030, 1021, 384)])
+def test_product_scales_at_any_address(qlib, dev, M, N, K):
+    """Scales whose rows start on no word boundary, at every offset."""
+    a, sa, b, sb = _operands(qlib, dev, M, N, K, False, False, 9)
+    c, want = torch.empty(M, N, device=dev), torch.empty(M, N, device=dev)
+    qlib.fp8_block_mm_e8m0(a, b, sa, sb, want)
+    for off in (1, 2, 3):
+        moved = []
+        for s in (sa, sb):
+            buf = torch.full((s.numel() + 8,), 255, dtype=torch.uint8, device=dev)
+            m = buf[off:off + s.numel()].view(s.shape)
+            m.copy_(s.view(torch.uint8))
+            moved.append(m.view(E8M0))
+        qlib.fp8_block_mm_e8m0(a, b, *moved, c)
+        assert torch.equal(c, want)
+
+
 def test_product_empty(qlib, dev):
     e = lambda r, c: qlib.quantize_block(torch.ones(r, c, device=dev))  # noqa: E731
     for M, N, K in ((0, 128, 128), (128, 0, 128), (5, 7, 0)):

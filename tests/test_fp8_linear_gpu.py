@@ -209,6 +209,26 @@ def test_capture_beside_a_living_graph_is_refused(qlib, dev):
     assert torch.equal(w.grad, want)
 
 
+def test_capture_beside_a_graph_of_another_side_stream(qlib, dev):
+    """Only the default stream's graphs hinder a capture."""
+    from qgemm_b200.linear import fp8_linear
+    x = _data(20, 256, torch.bfloat16, dev, 1)
+    w = _data(40, 256, torch.float32, dev, 2).requires_grad_(True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        alive = fp8_linear(x, w)
+        want, = torch.autograd.grad(fp8_linear(x, w).sum(), w)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got, = torch.autograd.grad(fp8_linear(x, w).sum(), w)
+        got.zero_()
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    del alive
+
+
 def test_two_streams_at_once(qlib, dev):
     """The operators share no scratch: layers on two streams, nothing ordering them, each get their own results."""
     from qgemm_b200.linear import fp8_linear
