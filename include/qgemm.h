@@ -166,6 +166,8 @@ int qgemm_dequantize_block(int out_dtype, const void* q, size_t ld_q, const void
  *   forward product and, on column forms, both backward products.
  *   accumulate != 0: the product is added to C, FP32 only (a gradient over several micro-batches).
  *   A [M,K], B [N,K]: 16-byte aligned bases and leading dimensions that are multiples of 16; C: any ldc >= N.
+ * An FP32 C over a long K (more than 6144 in one chain of the tensor cores, whose additions truncate) is made in several
+ * launches that add up, so that its relative error stays below 1e-6.
  * Any M, N, K >= 0 (K = 0: zeros, or C unchanged when accumulating). No library scratch is used, so calls on several
  * streams are independent; results are reproducible. The first GEMM call on a device must not be inside a stream capture.
  */

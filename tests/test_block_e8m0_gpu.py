@@ -332,6 +332,25 @@ def test_product_nan_blocks_reach_their_rows_only(qlib, dev):
     assert torch.equal(torch.isnan(c), bad)
 
 
+@pytest.mark.parametrize("M,N,K", [(16, 128, 70000), (256, 256, 40001), (600, 700, 16500), (1000, 1100, 6145)])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_long_sums_keep_32_bits(qlib, dev, M, N, K, accumulate):
+    """A fp32 result's error does not grow with K. The tensor cores' additions truncate; over one chain of 8192 signed terms
+    that was measured as 8.6e-7 of the result's norm, in proportion to the length, so the 6144 that a chain may have lose
+    6.5e-7, and parts that are added with a rounding each lose no more than that together. 1e-6 leaves half as much again;
+    one chain over the longest K here would be 1.3e-5 off."""
+    a, sa, b, sb = _operands(qlib, dev, M, N, K, False, False, 21, 0.5)
+    ref, mags = _product(a, sa, b, sb)
+    c = torch.randn(M, N, device=dev) * float(ref.abs().mean()) if accumulate else torch.empty(M, N, device=dev)
+    want = ref + c.double() if accumulate else ref
+    qlib.fp8_block_mm_e8m0(a, b, sa, sb, c, accumulate=accumulate)
+    assert float((c.double() - want).norm() / want.norm()) <= 1e-6
+    again = c.clone()
+    if not accumulate:
+        qlib.fp8_block_mm_e8m0(a, b, sa, sb, again)
+        assert torch.equal(again, c)
+
+
 @pytest.mark.parametrize("M,N,K", [(5, 300, 1000), (333, 259, 700), (1030, 1021, 384)])
 def test_product_scales_at_any_address(qlib, dev, M, N, K):
     """Scales whose rows start on no word boundary, at every offset."""
