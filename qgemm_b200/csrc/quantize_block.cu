@@ -26,6 +26,8 @@ namespace {
 constexpr int kQbThreads = 256;
 constexpr int kQb = 128;  // block length, and the side of a CTA's tile
 
+enum : int { kAnywhere = 0, kEights = 1, kVectors = 2 };
+
 struct QuantBlockParams {
     const void* in;
     long long ld_in;
@@ -34,7 +36,8 @@ struct QuantBlockParams {
     long long ld_q, ld_qt;
     uint8_t *scale, *scale_t;  // [ceil(cols/128), rows or ceil(rows/128)], [ceil(rows/128), cols or ceil(cols/128)]
     int rows, cols;
-    int vec_in, vec_q, vec_qt;  // 8 elements can be loaded, 8 codes stored, in whole vectors
+    int source;         // what the source's rows are aligned to
+    int vec_q, vec_qt;  // 8 codes can be stored in whole vectors
 };
 
 // Scale byte from the bit pattern of max |x| (infinities and NaN order above every number).
@@ -68,6 +71,22 @@ struct Eight<float> {
         const uint4 a = __ldg(reinterpret_cast<const uint4*>(p)), b = __ldg(reinterpret_cast<const uint4*>(p) + 1);
         w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w; w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
     }
+    __device__ __forceinline__ void load_by_eights(const float* p) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const uint2 a = __ldg(reinterpret_cast<const uint2*>(p) + k);
+            w[2 * k] = a.x;
+            w[2 * k + 1] = a.y;
+        }
+    }
+    __device__ __forceinline__ void load_any(const float* p) {
+        if ((reinterpret_cast<uintptr_t>(p) & 7u) == 0) {
+            load_by_eights(p);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) w[k] = __ldg(reinterpret_cast<const uint32_t*>(p) + k);
+        }
+    }
     __device__ __forceinline__ void set(int j, const float* p) { w[j] = __ldg(reinterpret_cast<const uint32_t*>(p)); }
     __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -87,6 +106,21 @@ struct Eight16 {
     __device__ __forceinline__ void load(const uint16_t* p) {
         const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
         w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+    }
+    __device__ __forceinline__ void load_by_eights(const uint16_t* p) {
+        const uint2 a = __ldg(reinterpret_cast<const uint2*>(p)), b = __ldg(reinterpret_cast<const uint2*>(p) + 1);
+        w[0] = a.x; w[1] = a.y; w[2] = b.x; w[3] = b.y;
+    }
+    // from any address: the words that hold the elements, shifted by half a word where they start inside one
+    __device__ __forceinline__ void load_any(const uint16_t* p) {
+        const uint32_t half = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) >> 1) & 1u;
+        const uint32_t* words = reinterpret_cast<const uint32_t*>(p - half);
+        uint32_t v[5];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = __ldg(words + k);
+        v[4] = __ldg(words + 3 + half);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = __funnelshift_r(v[k], v[k + 1], 16u * half);
     }
     __device__ __forceinline__ void set(int j, const uint16_t* p) {
         const uint32_t v = __ldg(p);
@@ -208,9 +242,9 @@ struct QuantShared {
 };
 
 // A thread's place in the tile: rows 8 * piece .. + 8 with piece = 0..15, columns 8 * cgroup .. + 8 with cgroup = lane & 15;
-// a load instruction of a warp covers two rows of 128 elements. WHOLE: the tile lies inside the matrix and everything is
-// aligned to whole vectors.
-template <typename T, bool ROW, bool COL, bool SQUARE, bool WHOLE>
+// a load instruction of a warp covers two rows of 128 elements. WHOLE: the tile lies inside the matrix and the codes are
+// aligned to whole vectors. SOURCE: what the source's rows are aligned to, vectors of 16 bytes, eight bytes or nothing.
+template <typename T, bool ROW, bool COL, bool SQUARE, bool WHOLE, int SOURCE>
 __device__ __forceinline__ void quantize_tile(const QuantBlockParams& p, QuantShared<COL, SQUARE>& sh) {
     using E = typename Elem<T>::type;
     using V = Eight<T>;
@@ -224,8 +258,12 @@ __device__ __forceinline__ void quantize_tile(const QuantBlockParams& p, QuantSh
     V v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i, src += p.ld_in) {
-        if (WHOLE || (r0 + i < p.rows && n_cols == 8 && p.vec_in)) {
+        if (WHOLE && SOURCE == kVectors) {
             v[i].load(src);
+        } else if (WHOLE && SOURCE == kEights) {
+            v[i].load_by_eights(src);
+        } else if (WHOLE || (r0 + i < p.rows && n_cols == 8)) {
+            v[i].load_any(src);
         } else {
             v[i].clear();
             if (r0 + i < p.rows) {
@@ -337,7 +375,7 @@ __device__ __forceinline__ void quantize_tile(const QuantBlockParams& p, QuantSh
 }
 
 __device__ __forceinline__ bool whole_tile(const QuantBlockParams& p) {
-    return p.vec_in && p.vec_q && p.vec_qt && static_cast<int>(blockIdx.y + 1) * kQb <= p.rows &&
+    return p.vec_q && p.vec_qt && static_cast<int>(blockIdx.y + 1) * kQb <= p.rows &&
            static_cast<int>(blockIdx.x + 1) * kQb <= p.cols;
 }
 
@@ -356,8 +394,10 @@ quantize_block_kernel(const QuantBlockParams p) {
     ptx::pdl_launch_dependents();
     ptx::pdl_wait();
     __shared__ __align__(16) QuantShared<COL, SQUARE> sh;
-    if (whole_tile(p)) quantize_tile<T, ROW, COL, SQUARE, true>(p, sh);
-    else quantize_tile<T, ROW, COL, SQUARE, false>(p, sh);
+    if (!whole_tile(p)) quantize_tile<T, ROW, COL, SQUARE, false, kAnywhere>(p, sh);
+    else if (p.source == kVectors) quantize_tile<T, ROW, COL, SQUARE, true, kVectors>(p, sh);
+    else if (p.source == kEights) quantize_tile<T, ROW, COL, SQUARE, true, kEights>(p, sh);
+    else quantize_tile<T, ROW, COL, SQUARE, true, kAnywhere>(p, sh);
 }
 
 // ------------------------------------------------------------------------------------------------ from 8 bits
@@ -416,7 +456,7 @@ __device__ __forceinline__ void load_codes(const QuantBlockParams& p, int r0, in
     const int n_cols = WHOLE ? 8 : min(8, p.cols - c0);
 #pragma unroll
     for (int i = 0; i < 8; ++i, src += p.ld_in) {
-        if (WHOLE || (r0 + i < p.rows && n_cols == 8 && p.vec_in)) {
+        if (WHOLE || (r0 + i < p.rows && n_cols == 8 && p.source == kEights)) {
             v[i] = __ldg(reinterpret_cast<const uint2*>(src));
         } else {
             v[i] = make_uint2(0u, 0u);
@@ -610,24 +650,38 @@ requantize_block_kernel(const QuantBlockParams p) {
     ptx::pdl_launch_dependents();
     ptx::pdl_wait();
     __shared__ __align__(16) RequantShared sh;
-    if (whole_tile(p)) requantize_tile<true>(p, sh);
+    if (p.source == kEights && whole_tile(p)) requantize_tile<true>(p, sh);
     else requantize_tile<false>(p, sh);
 }
 
 // out = round(code * 2^E). The product is exact in fp32 (or overflows to an infinity, as the rounded value does), so the
 // conversion to the output type is the one rounding. A thread has W neighbouring columns (16 bytes of output) of four rows
-// at a time (eight took more registers: 16384 x 7168 to bf16 75 us instead of 59): their loads are all in flight together, a warp's stores cover whole lines, and rows and columns come without a
-// division.
-constexpr int kDequantRows = 4;
+// at a time (eight took more registers: 16384 x 7168 to bf16 75 us instead of 59): their loads are all in flight together, a
+// warp's stores cover whole lines, and rows and columns come without a division. Where rows of `out` do not start on 16
+// bytes (VEC false) an fp32 thread stores its columns one by one, and a 16-bit thread has two columns of eight rows, a word
+// of output where a row starts on one (4001 x 7167 to bf16: by eight single columns 80 us, by one 52).
 template <int OUT>
+__device__ __forceinline__ void store_value(uint8_t* dst, float x) {
+    if constexpr (OUT == OUT_F32) *reinterpret_cast<float*>(dst) = x;
+    else if constexpr (OUT == OUT_BF16) *reinterpret_cast<__nv_bfloat16*>(dst) = __float2bfloat16_rn(x);
+    else *reinterpret_cast<__half*>(dst) = __float2half_rn(x);
+}
+__device__ __forceinline__ float scale_value(uint32_t byte) {
+    return byte == 255u ? __uint_as_float(0x7fffffffu) : (byte == 0u ? __uint_as_float(0x400000u) : __uint_as_float(byte << 23));
+}
+template <int OUT, bool VEC>
+struct DequantShape {
+    static constexpr int kCols = OUT == OUT_F32 ? 4 : (VEC ? 8 : 2);
+    static constexpr int kRows = OUT == OUT_F32 || VEC ? 4 : 8;
+};
+template <int OUT, bool VEC>
 __global__ void __launch_bounds__(kQbThreads, 4)
 dequantize_block_kernel(const uint8_t* __restrict__ q, long long ld_q, const uint8_t* __restrict__ scale, int block_shift,
-                        long long scale_rows, int rows, int cols, uint8_t* __restrict__ out, long long ld_out, int vec_in,
-                        int vec_out) {
+                        long long scale_rows, int rows, int cols, uint8_t* __restrict__ out, long long ld_out, int vec_in) {
     ptx::pdl_launch_dependents();
     ptx::pdl_wait();
     constexpr int OB = OUT == OUT_F32 ? 4 : 2;
-    constexpr int W = 16 / OB, U = kDequantRows;
+    constexpr int W = DequantShape<OUT, VEC>::kCols, U = DequantShape<OUT, VEC>::kRows;
     const int c = (static_cast<int>(blockIdx.x) * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x)) * W;
     if (c >= cols) return;
     const int n = min(W, cols - c);
@@ -636,68 +690,90 @@ dequantize_block_kernel(const uint8_t* __restrict__ q, long long ld_q, const uin
     for (long long r0 = (static_cast<long long>(blockIdx.y) * blockDim.y + threadIdx.y) * U; r0 < rows; r0 += step) {
         const int nr = static_cast<int>(min(static_cast<long long>(U), rows - r0));
         const uint8_t* src = q + r0 * ld_q + c;
-        uint32_t v[U][W / 4], byte[U];
+        if constexpr (W == 2) {
+            uint32_t code[U], byte[U];
 #pragma unroll
-        for (int i = 0; i < U; ++i) {
+            for (int i = 0; i < U; ++i) {
+                const int k = min(i, nr - 1);
+                const uint8_t* at = src + k * ld_q;
+                if (vec_in && n == 2) code[i] = __ldg(reinterpret_cast<const uint16_t*>(at));
+                else code[i] = __ldg(at) | (n == 2 ? static_cast<uint32_t>(__ldg(at + 1)) << 8 : 0u);
+                byte[i] = __ldg(scales + ((r0 + k) >> block_shift));
+            }
+            uint8_t* dst = out + (r0 * ld_out + c) * OB;
 #pragma unroll
-            for (int k = 0; k < W / 4; ++k) v[i][k] = 0u;
-            byte[i] = 127u;
-            if (i < nr) {
-                byte[i] = __ldg(scales + ((r0 + i) >> block_shift));
-                if (n == W && vec_in) {
-                    if constexpr (W == 8) {
-                        const uint2 w = __ldg(reinterpret_cast<const uint2*>(src + i * ld_q));
-                        v[i][0] = w.x;
-                        v[i][1] = w.y;
+            for (int i = 0; i < U; ++i, dst += ld_out * OB) {
+                if (i >= nr) continue;
+                const float2 x = __half22float2(decode2(code[i]));
+                const float s = scale_value(byte[i]);
+                if (n == 2 && (reinterpret_cast<uintptr_t>(dst) & 3u) == 0) {
+                    uint32_t u;
+                    if constexpr (OUT == OUT_BF16) {
+                        const __nv_bfloat162 h = __floats2bfloat162_rn(x.x * s, x.y * s);
+                        u = *reinterpret_cast<const uint32_t*>(&h);
                     } else {
-                        v[i][0] = __ldg(reinterpret_cast<const uint32_t*>(src + i * ld_q));
+                        u = bits_of(__floats2half2_rn(x.x * s, x.y * s));
                     }
+                    *reinterpret_cast<uint32_t*>(dst) = u;
                 } else {
-#pragma unroll
-                    for (int j = 0; j < W; ++j)
-                        if (j < n) v[i][j >> 2] |= static_cast<uint32_t>(__ldg(src + i * ld_q + j)) << (8 * (j & 3));
+                    store_value<OUT>(dst, x.x * s);
+                    if (n == 2) store_value<OUT>(dst + OB, x.y * s);
                 }
             }
-        }
+            continue;
+        } else {
+            uint32_t v[U][W / 4], byte[U];
 #pragma unroll
-        for (int i = 0; i < U; ++i) {
-            if (i >= nr) break;
-            const float s = byte[i] == 255u ? __uint_as_float(0x7fffffffu)
-                                            : (byte[i] == 0u ? __uint_as_float(0x400000u) : __uint_as_float(byte[i] << 23));
-            float x[W];
+            for (int i = 0; i < U; ++i) {
 #pragma unroll
-            for (int k = 0; k < W / 4; ++k) decode4(v[i][k], *reinterpret_cast<float(*)[4]>(&x[4 * k]));
-#pragma unroll
-            for (int j = 0; j < W; ++j) x[j] *= s;
-            uint8_t* dst = out + ((r0 + i) * ld_out + c) * OB;
-            if constexpr (OUT == OUT_F32) {
-                if (n == W && vec_out) {
-                    *reinterpret_cast<float4*>(dst) = make_float4(x[0], x[1], x[2], x[3]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < W; ++j)
-                        if (j < n) reinterpret_cast<float*>(dst)[j] = x[j];
-                }
-            } else {
-                uint32_t u[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if constexpr (OUT == OUT_BF16) {
-                        const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
-                        u[j] = *reinterpret_cast<const uint32_t*>(&h);
+                for (int k = 0; k < W / 4; ++k) v[i][k] = 0u;
+                byte[i] = 127u;
+                if (i < nr) {
+                    byte[i] = __ldg(scales + ((r0 + i) >> block_shift));
+                    if (n == W && vec_in) {
+                        if constexpr (W == 8) {
+                            const uint2 w = __ldg(reinterpret_cast<const uint2*>(src + i * ld_q));
+                            v[i][0] = w.x;
+                            v[i][1] = w.y;
+                        } else {
+                            v[i][0] = __ldg(reinterpret_cast<const uint32_t*>(src + i * ld_q));
+                        }
                     } else {
-                        const __half2 h = __floats2half2_rn(x[2 * j], x[2 * j + 1]);
-                        u[j] = *reinterpret_cast<const uint32_t*>(&h);
+#pragma unroll
+                        for (int j = 0; j < W; ++j)
+                            if (j < n) v[i][j >> 2] |= static_cast<uint32_t>(__ldg(src + i * ld_q + j)) << (8 * (j & 3));
                     }
                 }
-                if (n == W && vec_out) {
-                    *reinterpret_cast<uint4*>(dst) = make_uint4(u[0], u[1], u[2], u[3]);
-                } else {
+            }
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                if (i >= nr) break;
+                const float s = scale_value(byte[i]);
+                float x[W];
+#pragma unroll
+                for (int k = 0; k < W / 4; ++k) decode4(v[i][k], *reinterpret_cast<float(*)[4]>(&x[4 * k]));
+#pragma unroll
+                for (int j = 0; j < W; ++j) x[j] *= s;
+                uint8_t* dst = out + ((r0 + i) * ld_out + c) * OB;
+                if (n < W || !VEC) {
 #pragma unroll
                     for (int j = 0; j < W; ++j)
-                        if (j < n)
-                            reinterpret_cast<uint16_t*>(dst)[j] =
-                                static_cast<uint16_t>((j & 1) ? (u[j >> 1] >> 16) : (u[j >> 1] & 0xffffu));
+                        if (j < n) store_value<OUT>(dst + j * OB, x[j]);
+                } else if constexpr (OUT == OUT_F32) {
+                    *reinterpret_cast<float4*>(dst) = make_float4(x[0], x[1], x[2], x[3]);
+                } else {
+                    uint32_t u[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if constexpr (OUT == OUT_BF16) {
+                            const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
+                            u[j] = *reinterpret_cast<const uint32_t*>(&h);
+                        } else {
+                            const __half2 h = __floats2half2_rn(x[2 * j], x[2 * j + 1]);
+                            u[j] = *reinterpret_cast<const uint32_t*>(&h);
+                        }
+                    }
+                    *reinterpret_cast<uint4*>(dst) = make_uint4(u[0], u[1], u[2], u[3]);
                 }
             }
         }
@@ -748,7 +824,7 @@ int quantize_block_launch(int in_dtype, const void* in, size_t ld_in, size_t row
     p.scale_t = scale_t;
     p.rows = static_cast<int>(rows);
     p.cols = static_cast<int>(cols);
-    p.vec_in = aligned(in, ld_in * es, 16);
+    p.source = aligned(in, ld_in * es, 16) ? kVectors : (aligned(in, ld_in * es, 8) ? kEights : kAnywhere);
     p.vec_q = q == nullptr || aligned(q, ld_q, 8);
     p.vec_qt = qt == nullptr || aligned(qt, ld_qt, 8);
     const dim3 grid(static_cast<unsigned>((cols + kQb - 1) / kQb), static_cast<unsigned>((rows + kQb - 1) / kQb));
@@ -776,7 +852,7 @@ int requantize_block_launch(const void* q, size_t ld_q, const uint8_t* scale, si
     p.scale_t = scale_t;
     p.rows = static_cast<int>(rows);
     p.cols = static_cast<int>(cols);
-    p.vec_in = aligned(q, ld_q, 8);
+    p.source = aligned(q, ld_q, 8) ? kEights : kAnywhere;
     p.vec_q = 1;
     p.vec_qt = aligned(qt, ld_qt, 8);
     const dim3 grid(static_cast<unsigned>((cols + kQb - 1) / kQb), static_cast<unsigned>((rows + kQb - 1) / kQb));
@@ -793,25 +869,29 @@ int dequantize_block_launch(int out_dtype, const void* q, size_t ld_q, const uin
     if (rows > kMaxSide || cols > kMaxSide) return QGEMM_ERR_INVALID_ARG;
     const size_t es = out_dtype == QGEMM_DTYPE_FP32 ? 4 : 2;
     if (reinterpret_cast<uintptr_t>(out) % es != 0) return QGEMM_ERR_ALIGNMENT;
+    const long long scale_rows = static_cast<long long>(block_rows == kQb ? (rows + kQb - 1) / kQb : rows);
+    const int shift = block_rows == kQb ? 7 : 0;
+    const bool vec_out = aligned(out, ld_out * es, 16);
+    const int vec_in = aligned(q, ld_q, es == 4 ? 4 : (vec_out ? 8 : 2));
     // a block: as many neighbouring pieces of a row as there are, up to 256, and rows for the rest of its threads
-    const size_t pieces = (cols + 16 / es - 1) / (16 / es);
+    const size_t piece = es == 4 ? 4 : (vec_out ? 8 : 2), rows_at_once = es == 4 || vec_out ? 4 : 8;
+    const size_t pieces = (cols + piece - 1) / piece;
     unsigned bx = 1;
     while (bx < static_cast<unsigned>(kQbThreads) && bx < pieces) bx *= 2;
     const unsigned by = kQbThreads / bx;
-    const size_t block_rows_at_once = static_cast<size_t>(by) * kDequantRows;
-    const size_t row_steps = (rows + block_rows_at_once - 1) / block_rows_at_once;
+    const size_t row_steps = (rows + by * rows_at_once - 1) / (by * rows_at_once);
     const dim3 grid(static_cast<unsigned>((pieces + bx - 1) / bx), static_cast<unsigned>(row_steps < 65535 ? row_steps : 65535));
-    const long long scale_rows = static_cast<long long>(block_rows == kQb ? (rows + kQb - 1) / kQb : rows);
-    const int shift = block_rows == kQb ? 7 : 0;
-    const int vec_in = aligned(q, ld_q, 16 / es), vec_out = aligned(out, ld_out * es, 16);
-    auto go = [&](auto kernel) {
-        return launch_pdl(kernel, grid, dim3(bx, by), 0, stream, static_cast<const uint8_t*>(q),
+    auto go = [&](auto vec_kernel, auto any_kernel) {
+        return launch_pdl(vec_out ? vec_kernel : any_kernel, grid, dim3(bx, by), 0, stream, static_cast<const uint8_t*>(q),
                           static_cast<long long>(ld_q), scale, shift, scale_rows, static_cast<int>(rows),
-                          static_cast<int>(cols), static_cast<uint8_t*>(out), static_cast<long long>(ld_out), vec_in, vec_out);
+                          static_cast<int>(cols), static_cast<uint8_t*>(out), static_cast<long long>(ld_out), vec_in);
     };
-    const cudaError_t e = out_dtype == QGEMM_DTYPE_FP32   ? go(dequantize_block_kernel<OUT_F32>)
-                          : out_dtype == QGEMM_DTYPE_BF16 ? go(dequantize_block_kernel<OUT_BF16>)
-                                                          : go(dequantize_block_kernel<OUT_F16>);
+    cudaError_t e;
+    switch (out_dtype) {
+        case QGEMM_DTYPE_FP32: e = go(dequantize_block_kernel<OUT_F32, true>, dequantize_block_kernel<OUT_F32, false>); break;
+        case QGEMM_DTYPE_BF16: e = go(dequantize_block_kernel<OUT_BF16, true>, dequantize_block_kernel<OUT_BF16, false>); break;
+        default: e = go(dequantize_block_kernel<OUT_F16, true>, dequantize_block_kernel<OUT_F16, false>); break;
+    }
     return e == cudaSuccess ? QGEMM_OK : QGEMM_ERR_CUDA;
 }
 
