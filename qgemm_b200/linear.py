@@ -184,9 +184,9 @@ def fp8_linear_forward(x, weight, need_dx: bool = True, need_dw: bool = True, ou
     if not packed:
         w_form = _Form(at, out_features, in_features, True)
         at = w_form.end
-    buffer = torch.empty(kept, dtype=torch.uint8, device=device) if kept else None
+    buffer = torch.empty(kept, dtype=torch.uint8, device=device) if need_dw or wt_form is not None else None
     scratch = torch.empty(at - kept, dtype=torch.uint8, device=device) if at > kept else None
-    base = buffer.data_ptr() if kept else 0
+    base = buffer.data_ptr() if buffer is not None else 0
     scratch_base = scratch.data_ptr() - kept if at > kept else 0
     x_base = base if need_dw else scratch_base
     if packed:

@@ -146,6 +146,14 @@ def test_checkpoint_restores_the_activation(qlib, dev):
     assert torch.equal(back.cpu(), _q(x).to(torch.float32).to(torch.bfloat16))
 
 
+def test_checkpoint_of_no_tokens_and_none_kept(qlib, dev):
+    from qgemm_b200.linear import fp8_linear_forward
+    x, w = _data(5, 512, torch.bfloat16, dev, 1), _data(130, 512, torch.bfloat16, dev, 2)
+    codes, scale = fp8_linear_forward(x[:0], w, need_dx=False)[1].x
+    assert codes.shape == (0, 512) and scale.shape == (4, 0)
+    assert fp8_linear_forward(x, w, need_dw=False)[1].x is None
+
+
 def _captured(step):
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
