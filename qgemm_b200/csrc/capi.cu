@@ -1119,9 +1119,8 @@ int e8m0_launch(const E8m0Plan& plan, const void* A, size_t lda, const void* B, 
     if (c_addr % 16 == 0 && (static_cast<size_t>(p.ldc) * out_bytes) % 16 == 0 && g_env.direct_store == 0)
         p.c_tma_ok = encode_output_map(p.C, p.M, p.N, p.ldc, 1, p.out, &tc) == QGEMM_OK ? 1 : 0;
     // tile rows walked together, so that their panels of A (16 MB of them) stay in L2 while B passes
-    p.group_m = g_env.group_m > 0
-                    ? g_env.group_m
-                    : static_cast<int>(std::max<long long>(4, std::min<long long>(4096, (16ll << 20) / (128ll * p.kb_total * 256))));
+    p.group_m = static_cast<int>(std::max<long long>(4, (16ll << 20) / (128ll * p.kb_total * 256)));
+    p.group_m = std::min(g_env.group_m > 0 ? g_env.group_m : p.group_m, p.m_tiles);
     p.idesc = ptx::make_idesc_e8m0(256u, static_cast<uint32_t>(plan.tile_n));
     const int clusters = static_cast<int>(std::min<long long>(tiles, sms / 2));
     return launch_e8m0_pair(plan.tile_n, plan.slices, ta, tb, tc, p, clusters, stream) == cudaSuccess ? QGEMM_OK : QGEMM_ERR_CUDA;
@@ -1174,7 +1173,8 @@ int e8m0_dispatch(int out_dtype, const void* A, size_t lda, const uint8_t* a_sca
     // The tensor cores' additions cut off what fp32 does not hold instead of rounding it, so a sum's error grows with its
     // length in one direction: measured against 64 bits 1.8e-7 relative over K = 2048, 8.6e-7 over 8192, 2.0e-6 over 16384 and
     // 1.3e-5 over 65536. No 16-bit result shows that. For a fp32 one, K is taken in parts of at most kE8ChainBlocks blocks a
-    // slice, the later ones added to C with one rounding each: below 7e-7 however long K is.
+    // slice, the later ones added to C with one rounding each: below 7e-7 however long K is. (A part has at least half of
+    // that, so every slice of its form has blocks.)
     const int kb = (p.K + 127) / 128;
     E8m0Plan plan = plan_e8m0(M, N, K, st->sm_count);
     int parts = 1;

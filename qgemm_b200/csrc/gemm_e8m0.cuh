@@ -118,9 +118,9 @@ __device__ __forceinline__ void put_scales(uint32_t dst, const ScaleWords& c, co
 
 // The four scale warps, over the chunks of K blocks [kb0, kb1) of work items first, first + step, ... < last. Unit u = 0 ..
 // UNITS - 1 is 128 rows of an operand, loaded by scale warp u from row rows(work item). `start` sends the first loads on their
-// way; `run` needs tensor memory, and is executed by all four warps to the end whatever
-// happens, because they meet at a barrier of their own for every chunk: after a wait that ran out they only meet. (`start` may
-// come before the CTA-wide barrier of a kernel whose other warps wait there for memory too.)
+// way, before the CTA-wide barrier in a kernel whose producer waits for memory there too. `run` needs tensor memory, and is
+// executed by all four warps to the end whatever happens, because they meet at a barrier of their own for every chunk: after
+// a wait that ran out they only meet.
 template <int UNITS>
 struct ScaleFeeder {
     ScaleSource src;

@@ -380,8 +380,8 @@ __device__ __forceinline__ bool whole_tile(const QuantBlockParams& p) {
 }
 
 // Tiles that share an SM, by the registers a tile can be held in: what a CTA has in flight is its tile, so this sets the
-// bandwidth. (16-bit, 4096 x 7168, column form: four 16.4 us,
-// two 21.3, five, with spilled registers, 18.7; both forms: three 22.3, two 25.9, four 23.2.)
+// bandwidth. (16-bit, 4096 x 7168, column form: four 16.4 us, two 21.3, five, with spilled registers, 18.7; both forms:
+// three 22.3, two 25.9, four 23.2.)
 template <typename T, bool ROW, bool COL, bool SQUARE>
 constexpr int tiles_per_sm() {
     if (sizeof(typename Elem<T>::type) == 2) return SQUARE ? (ROW ? 4 : 5) : (ROW && COL ? 3 : 4);
