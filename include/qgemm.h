@@ -164,7 +164,8 @@ int qgemm_dequantize_block(int out_dtype, const void* q, size_t ld_q, const void
  *   with 128-wide K blocks, ea = a_scale[kb*M + m] (a_block_rows = 1) or a_scale[kb*ceil(M/128) + m/128] (128), and eb the
  *   same of B and N; fp32 accumulation, one rounding to out_dtype (BF16, FP16 or FP32). The same entry serves a layer's
  *   forward product and, on column forms, both backward products.
- *   accumulate != 0: the product is added to C, FP32 only (a gradient over several micro-batches).
+ *   accumulate != 0: the product is added to C, FP32 only (a gradient over several micro-batches). The additions are made
+ *   by the memory system, which takes numbers below 2^-126 as zeros.
  *   A [M,K], B [N,K]: 16-byte aligned bases and leading dimensions that are multiples of 16; C: any ldc >= N.
  * An FP32 C over a long K (more than 6144 in one chain of the tensor cores, whose additions truncate) is made in several
  * launches that add up, so that its relative error stays below 1e-6.

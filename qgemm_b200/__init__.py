@@ -500,7 +500,7 @@ def fp8_block_mm_e8m0(a, b, a_scale, b_scale, c, accumulate: bool = False) -> No
     """c[m,n] = a[m,k] x b[n,k]^T of FP8 codes with power-of-two block scales (:func:`quantize_block`), the scales applied
     by the tensor cores; argument order as :func:`fp8_block_mm`. ``a_scale`` [ceil(k/128), m] or, one for 128 rows,
     [ceil(k/128), ceil(m/128)]; ``b_scale`` likewise of n. ``c`` bf16 / fp16 / fp32; ``accumulate`` adds to what a fp32 ``c``
-    holds. Rows of ``a`` and ``b`` start on 16-byte boundaries. A layer's three products, with x, w and dy quantised:
+    holds (numbers below 2^-126 count as zeros there). Rows of ``a`` and ``b`` start on 16-byte boundaries. A layer's three products, with x, w and dy quantised:
     forward (x row, w row), dx = (dy row, w column), dw = (dy column, x column)."""
     M, K, lda = _codes("a", a)
     N, Kb, ldb = _codes("b", b)

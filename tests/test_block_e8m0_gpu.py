@@ -269,6 +269,21 @@ def test_product_accumulates(qlib, dev, M, N, K):
     assert bool((wide[:, :3] == 3).all()) and bool((wide[:, N + 3:] == 3).all())
 
 
+@pytest.mark.parametrize("M,N,K", [(16, 512, 512), (300, 512, 256), (512, 512, 16384), (2048, 2048, 128)])
+def test_accumulating_takes_tiny_numbers_as_zeros(qlib, dev, M, N, K):
+    """On every way to C alike: vectors, rows, TMA. 2^-126 itself and what is larger stay."""
+    zeros = lambda r: torch.zeros(r, K, device=dev)  # noqa: E731
+    (a, sa), (b, sb) = qlib.quantize_block(zeros(M)), qlib.quantize_block(zeros(N), square=True)
+    old = torch.randint(0, 4, (M, N), device=dev)
+    held = torch.tensor([2.0 ** -126, 2.0 ** -127, -2.0 ** -149, -3.5], device=dev)
+    want = torch.tensor([2.0 ** -126, 0.0, 0.0, -3.5], device=dev)[old]
+    for off in (0, 1):
+        c = torch.empty(M * N + 4, device=dev)[off:off + M * N].view(M, N)
+        c.copy_(held[old])
+        qlib.fp8_block_mm_e8m0(a, b, sa, sb, c, accumulate=True)
+        assert torch.equal(c, want)
+
+
 @pytest.mark.parametrize("M,N,K", [(5, 300, 384), (300, 520, 1040), (2100, 2300, 256)])
 @pytest.mark.parametrize("out", TYPES)
 def test_product_strided(qlib, dev, M, N, K, out):
