@@ -76,7 +76,7 @@ __device__ __forceinline__ const uint8_t* scale_row(const ScaleSource& s, int ro
 __device__ __forceinline__ void load_scales(ScaleWords& out, const ScaleSource& s, int row0, int kb0, int n, int lane) {
     if (s.shift != 0) {  // one scale for the 128 rows
 #pragma unroll
-        for (int i = 0; i < 4; ++i) out.lo[i] = __ldg(scale_row(s, row0, kb0 + min(i, n - 1)));
+        for (int i = 0; i < 4; ++i) out.lo[i] = ptx::ld_global(scale_row(s, row0, kb0 + min(i, n - 1)));
         return;
     }
     const int bytes = min(128, s.rows - min(row0, s.rows - 1));
@@ -86,8 +86,8 @@ __device__ __forceinline__ void load_scales(ScaleWords& out, const ScaleSource& 
         const int off = static_cast<int>(reinterpret_cast<uintptr_t>(at) & 3u);
         const int last = (off + bytes - 1) >> 2;
         const uint32_t* words = reinterpret_cast<const uint32_t*>(at - off);
-        out.lo[i] = __ldg(words + min(lane, last));
-        if (off != 0) out.hi[i] = __ldg(words + min(lane + 1, last));
+        out.lo[i] = ptx::ld_global(words + min(lane, last));
+        if (off != 0) out.hi[i] = ptx::ld_global(words + min(lane + 1, last));
     }
 }
 // Into 512 bytes of shared memory: row r's four K blocks as a word at (r % 32) * 16 + (r / 32) * 4, so that lane l finds the

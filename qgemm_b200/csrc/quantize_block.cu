@@ -68,13 +68,14 @@ struct Eight<float> {
     uint32_t w[8];
     static constexpr int kWords = 8;  // one column a word
     __device__ __forceinline__ void load(const float* p) {
-        const uint4 a = __ldg(reinterpret_cast<const uint4*>(p)), b = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+        const uint4* at = reinterpret_cast<const uint4*>(p);
+        const uint4 a = ptx::ld_global(at), b = ptx::ld_global(at + 1);
         w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w; w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
     }
     __device__ __forceinline__ void load_by_eights(const float* p) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const uint2 a = __ldg(reinterpret_cast<const uint2*>(p) + k);
+            const uint2 a = ptx::ld_global(reinterpret_cast<const uint2*>(p) + k);
             w[2 * k] = a.x;
             w[2 * k + 1] = a.y;
         }
@@ -84,10 +85,10 @@ struct Eight<float> {
             load_by_eights(p);
         } else {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) w[k] = __ldg(reinterpret_cast<const uint32_t*>(p) + k);
+            for (int k = 0; k < 8; ++k) w[k] = ptx::ld_global(reinterpret_cast<const uint32_t*>(p) + k);
         }
     }
-    __device__ __forceinline__ void set(int j, const float* p) { w[j] = __ldg(reinterpret_cast<const uint32_t*>(p)); }
+    __device__ __forceinline__ void set(int j, const float* p) { w[j] = ptx::ld_global(reinterpret_cast<const uint32_t*>(p)); }
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int j = 0; j < 8; ++j) w[j] = 0u;
@@ -104,11 +105,12 @@ struct Eight16 {
     uint32_t w[4];
     static constexpr int kWords = 4;  // two columns a word
     __device__ __forceinline__ void load(const uint16_t* p) {
-        const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+        const uint4 a = ptx::ld_global(reinterpret_cast<const uint4*>(p));
         w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
     }
     __device__ __forceinline__ void load_by_eights(const uint16_t* p) {
-        const uint2 a = __ldg(reinterpret_cast<const uint2*>(p)), b = __ldg(reinterpret_cast<const uint2*>(p) + 1);
+        const uint2* at = reinterpret_cast<const uint2*>(p);
+        const uint2 a = ptx::ld_global(at), b = ptx::ld_global(at + 1);
         w[0] = a.x; w[1] = a.y; w[2] = b.x; w[3] = b.y;
     }
     // from any address: the words that hold the elements, shifted by half a word where they start inside one
@@ -117,13 +119,13 @@ struct Eight16 {
         const uint32_t* words = reinterpret_cast<const uint32_t*>(p - half);
         uint32_t v[5];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = __ldg(words + k);
-        v[4] = __ldg(words + 3 + half);
+        for (int k = 0; k < 4; ++k) v[k] = ptx::ld_global(words + k);
+        v[4] = ptx::ld_global(words + 3 + half);
 #pragma unroll
         for (int k = 0; k < 4; ++k) w[k] = __funnelshift_r(v[k], v[k + 1], 16u * half);
     }
     __device__ __forceinline__ void set(int j, const uint16_t* p) {
-        const uint32_t v = __ldg(p);
+        const uint32_t v = ptx::ld_global(p);
         w[j >> 1] |= v << (16 * (j & 1));
     }
     __device__ __forceinline__ void clear() {
@@ -457,12 +459,12 @@ __device__ __forceinline__ void load_codes(const QuantBlockParams& p, int r0, in
 #pragma unroll
     for (int i = 0; i < 8; ++i, src += p.ld_in) {
         if (WHOLE || (r0 + i < p.rows && n_cols == 8 && p.source == kEights)) {
-            v[i] = __ldg(reinterpret_cast<const uint2*>(src));
+            v[i] = ptx::ld_global(reinterpret_cast<const uint2*>(src));
         } else {
             v[i] = make_uint2(0u, 0u);
             if (r0 + i < p.rows) {
                 for (int j = 0; j < n_cols; ++j) {
-                    const uint32_t c = __ldg(src + j);
+                    const uint32_t c = ptx::ld_global(src + j);
                     if (j < 4) v[i].x |= c << (8 * j);
                     else v[i].y |= c << (8 * (j - 4));
                 }
@@ -484,7 +486,7 @@ __device__ __noinline__ void requantize_tile_fp32(const QuantBlockParams& p, Req
     uint32_t m[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        s[i] = shifted_scale(WHOLE || row0 + piece * 8 + i < p.rows ? __ldg(scales + i) : 127u);
+        s[i] = shifted_scale(WHOLE || row0 + piece * 8 + i < p.rows ? ptx::ld_global(scales + i) : 127u);
         float x[4];
         decode4(v[i].x, x);
 #pragma unroll
@@ -564,13 +566,13 @@ __device__ __forceinline__ void requantize_tile(const QuantBlockParams& p, Requa
     const uint8_t* scales = p.in_scale + static_cast<long long>(blockIdx.x) * p.rows + row0;
     const int own = piece * 8 + (cgroup >> 1);
     const bool exists = WHOLE || row0 + own < p.rows;
-    const uint32_t byte = exists ? __ldg(scales + own) : 0u;
+    const uint32_t byte = exists ? ptx::ld_global(scales + own) : 0u;
     uint32_t top = 0u, low = 255u;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const int r = 32 * j + lane;
         if (WHOLE || row0 + r < p.rows) {
-            const uint32_t b = __ldg(scales + r);
+            const uint32_t b = ptx::ld_global(scales + r);
             top = max(top, b);
             low = min(low, b);
         }
@@ -676,8 +678,8 @@ struct DequantShape {
 };
 template <int OUT, bool VEC>
 __global__ void __launch_bounds__(kQbThreads, 4)
-dequantize_block_kernel(const uint8_t* __restrict__ q, long long ld_q, const uint8_t* __restrict__ scale, int block_shift,
-                        long long scale_rows, int rows, int cols, uint8_t* __restrict__ out, long long ld_out, int vec_in) {
+dequantize_block_kernel(const uint8_t* q, long long ld_q, const uint8_t* scale, int block_shift, long long scale_rows, int rows,
+                        int cols, uint8_t* out, long long ld_out, int vec_in) {
     ptx::pdl_launch_dependents();
     ptx::pdl_wait();
     constexpr int OB = OUT == OUT_F32 ? 4 : 2;
@@ -696,9 +698,9 @@ dequantize_block_kernel(const uint8_t* __restrict__ q, long long ld_q, const uin
             for (int i = 0; i < U; ++i) {
                 const int k = min(i, nr - 1);
                 const uint8_t* at = src + k * ld_q;
-                if (vec_in && n == 2) code[i] = __ldg(reinterpret_cast<const uint16_t*>(at));
-                else code[i] = __ldg(at) | (n == 2 ? static_cast<uint32_t>(__ldg(at + 1)) << 8 : 0u);
-                byte[i] = __ldg(scales + ((r0 + k) >> block_shift));
+                if (vec_in && n == 2) code[i] = ptx::ld_global(reinterpret_cast<const uint16_t*>(at));
+                else code[i] = ptx::ld_global(at) | (n == 2 ? ptx::ld_global(at + 1) << 8 : 0u);
+                byte[i] = ptx::ld_global(scales + ((r0 + k) >> block_shift));
             }
             uint8_t* dst = out + (r0 * ld_out + c) * OB;
 #pragma unroll
@@ -729,19 +731,19 @@ dequantize_block_kernel(const uint8_t* __restrict__ q, long long ld_q, const uin
                 for (int k = 0; k < W / 4; ++k) v[i][k] = 0u;
                 byte[i] = 127u;
                 if (i < nr) {
-                    byte[i] = __ldg(scales + ((r0 + i) >> block_shift));
+                    byte[i] = ptx::ld_global(scales + ((r0 + i) >> block_shift));
                     if (n == W && vec_in) {
                         if constexpr (W == 8) {
-                            const uint2 w = __ldg(reinterpret_cast<const uint2*>(src + i * ld_q));
+                            const uint2 w = ptx::ld_global(reinterpret_cast<const uint2*>(src + i * ld_q));
                             v[i][0] = w.x;
                             v[i][1] = w.y;
                         } else {
-                            v[i][0] = __ldg(reinterpret_cast<const uint32_t*>(src + i * ld_q));
+                            v[i][0] = ptx::ld_global(reinterpret_cast<const uint32_t*>(src + i * ld_q));
                         }
                     } else {
 #pragma unroll
                         for (int j = 0; j < W; ++j)
-                            if (j < n) v[i][j >> 2] |= static_cast<uint32_t>(__ldg(src + i * ld_q + j)) << (8 * (j & 3));
+                            if (j < n) v[i][j >> 2] |= ptx::ld_global(src + i * ld_q + j) << (8 * (j & 3));
                     }
                 }
             }

@@ -1,0 +1,30 @@
+"""Block operators back to back on the same buffers, each kernel starting while the one that writes its operands still runs:
+every result equals that of the same calls with the device waited for in between."""
+import pytest
+import torch
+
+from test_block_e8m0_gpu import _data
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 2048, 4096), (40, 520, 1040), (300, 1024, 2048), (2304, 2176, 640)])
+def test_operands_rewritten_between_calls(qlib, dev, M, N, K):
+    sets = [(_data(M, K, torch.bfloat16, dev, 50 + i, 1.0), _data(N, K, torch.bfloat16, dev, 60 + i, 1.0)) for i in range(3)]
+    a, b = qlib.quantize_block(sets[0][0]), qlib.quantize_block(sets[0][1])
+    at = qlib.requantize_block(*a)
+    c, back = torch.empty(M, N, device=dev), torch.empty(M, K, dtype=torch.bfloat16, device=dev)
+
+    def step(x, w, between):
+        for call in (lambda: qlib.quantize_block(x, out=a), lambda: qlib.quantize_block(w, out=b),
+                     lambda: qlib.fp8_block_mm_e8m0(a[0], b[0], a[1], b[1], c), lambda: qlib.requantize_block(*a, out=at),
+                     lambda: qlib.dequantize_block(*a, out=back)):
+            call()
+            between()
+        return [t.clone() for t in (c, back, at[0].view(torch.uint8), at[1].view(torch.uint8))]
+
+    want = [step(x, w, torch.cuda.synchronize) for x, w in sets]
+    got = [step(x, w, lambda: None) for _ in range(10) for x, w in sets]
+    for i, outs in enumerate(got):
+        for g, r in zip(outs, want[i % 3]):
+            assert torch.equal(g, r), i
