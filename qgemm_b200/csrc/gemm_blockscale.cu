@@ -204,14 +204,14 @@ fp8_blockscale_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
 #pragma unroll
             for (int j = 0; j < CPW; ++j) acc[j] = 0.0f;
             // scales are fetched one K block ahead so that their latency never sits between a partial and its FMAs
-            float sa_next = row_ok ? __ldg(p.a_scale + row) : 0.0f;
-            float sb_next = __ldg(p.b_scale + n_blk);
+            float sa_next = row_ok ? ptx::ld_global(p.a_scale + row) : 0.0f;
+            float sb_next = ptx::ld_global(p.b_scale + n_blk);
             for (int kb = 0; kb < p.kb_total; ++kb, ++blk) {
                 const uint32_t buf = blk & PMASK;
                 const float sa = sa_next, sb = sb_next;
                 if (kb + 1 < p.kb_total) {
-                    sa_next = row_ok ? __ldg(p.a_scale + static_cast<long long>(kb + 1) * p.M + row) : 0.0f;
-                    sb_next = __ldg(p.b_scale + static_cast<long long>(kb + 1) * p.n_scale_blocks + n_blk);
+                    sa_next = row_ok ? ptx::ld_global(p.a_scale + static_cast<long long>(kb + 1) * p.M + row) : 0.0f;
+                    sb_next = ptx::ld_global(p.b_scale + static_cast<long long>(kb + 1) * p.n_scale_blocks + n_blk);
                 }
                 if (!wait_bounded(bar_done + slot * 8, slot_phase, abort_flag, p.status, ROLE_EPILOGUE, kb)) {
                     ok = false;

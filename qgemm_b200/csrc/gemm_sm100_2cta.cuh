@@ -215,8 +215,8 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
         const int quad = warp & 3;
         float alpha = 1.0f;
         if constexpr (OUT != OUT_RAW32) {
-            if (p.scale_a != nullptr) alpha *= __ldg(p.scale_a);
-            if (p.scale_b != nullptr) alpha *= __ldg(p.scale_b);
+            if (p.scale_a != nullptr) alpha *= ptx::ld_global(p.scale_a);
+            if (p.scale_b != nullptr) alpha *= ptx::ld_global(p.scale_b);
         }
         uint32_t it = 0;
         uint32_t out_buf = 0;

@@ -229,8 +229,8 @@ gemm_tcgen05_kcluster_kernel(const __grid_constant__ CUtensorMap tmap_a, const _
         const int n_valid = min(4, p.N - n0);
         float alpha = 1.0f;
         if constexpr (OUT != OUT_RAW32) {
-            if (p.scale_a != nullptr) alpha *= __ldg(p.scale_a);
-            if (p.scale_b != nullptr) alpha *= __ldg(p.scale_b);
+            if (p.scale_a != nullptr) alpha *= ptx::ld_global(p.scale_a);
+            if (p.scale_b != nullptr) alpha *= ptx::ld_global(p.scale_b);
         }
         constexpr int OB = OutBytes<OUT>::value;
         if (n_valid > 0) {

@@ -28,8 +28,8 @@ __device__ __forceinline__ void widen8(uint32_t w, uint32_t& lo4, uint32_t& hi4)
 // One thread widens 32 elements (16 packed bytes) of a row: blockIdx.x walks along the row, blockIdx.y strides over
 // the rows (no per-thread division).
 __global__ void __launch_bounds__(kUnpackThreads)
-unpack_int4_kernel(const uint8_t* __restrict__ in, long long ld_in_bytes, int8_t* __restrict__ out, long long ld_out,
-                   int rows, int cols, int vec_ok) {
+unpack_int4_kernel(const uint8_t* in, long long ld_in_bytes, int8_t* out, long long ld_out, int rows, int cols,
+                   int vec_ok) {
     ptx::pdl_launch_dependents();
     ptx::pdl_wait();
     const int c = (static_cast<int>(blockIdx.x) * kUnpackThreads + static_cast<int>(threadIdx.x)) * 32;
@@ -38,7 +38,7 @@ unpack_int4_kernel(const uint8_t* __restrict__ in, long long ld_in_bytes, int8_t
         const uint8_t* src = in + r * ld_in_bytes + c / 2;
         int8_t* dst = out + r * ld_out + c;
         if (vec_ok && c + 32 <= cols) {
-            const uint4 v = __ldg(reinterpret_cast<const uint4*>(src));
+            const uint4 v = ptx::ld_global(reinterpret_cast<const uint4*>(src));
             uint4 a, b;
             widen8(v.x, a.x, a.y);
             widen8(v.y, a.z, a.w);

@@ -33,7 +33,7 @@ __device__ __forceinline__ float load_as_float(const TIn* p) {
 template <typename TIn>
 struct Quad {
     using Raw = typename std::conditional<sizeof(TIn) == 4, float4, uint2>::type;
-    static __device__ __forceinline__ Raw load(const TIn* p) { return __ldg(reinterpret_cast<const Raw*>(p)); }
+    static __device__ __forceinline__ Raw load(const TIn* p) { return ptx::ld_global(reinterpret_cast<const Raw*>(p)); }
     static __device__ __forceinline__ void to_float(const Raw& v, float (&x)[4]) {
         if constexpr (sizeof(TIn) == 4) {
             x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
@@ -58,7 +58,7 @@ struct Unroll {
 // chunk, not one per element (a 64-bit division costs more than the rest of the per-element work together).
 template <typename TIn>
 __global__ void __launch_bounds__(kQuantThreads)
-amax_kernel(const TIn* __restrict__ in, long long ld, int rows, int cols, float* __restrict__ amax_out, int vec_ok) {
+amax_kernel(const TIn* in, long long ld, int rows, int cols, float* amax_out, int vec_ok) {
     ptx::pdl_launch_dependents();
     ptx::pdl_wait();
     constexpr int U = Unroll<TIn>::value;
@@ -190,13 +190,13 @@ __device__ __forceinline__ uint32_t quantize_quad(const float (&x)[4], const Quo
 
 template <typename TIn, bool FP8>
 __global__ void __launch_bounds__(kQuantThreads)
-quantize_kernel(const TIn* __restrict__ in, long long ld_in, uint8_t* __restrict__ out, long long ld_out, int rows,
-                int cols, const float* __restrict__ amax_in, float* __restrict__ scale_out, int vec_ok) {
+quantize_kernel(const TIn* in, long long ld_in, uint8_t* out, long long ld_out, int rows, int cols, const float* amax_in,
+                float* scale_out, int vec_ok) {
     ptx::pdl_launch_dependents();
     ptx::pdl_wait();
     constexpr int U = Unroll<TIn>::value;
     constexpr int kChunkQuads = kQuantThreads * U;
-    const float amax = __ldg(amax_in);
+    const float amax = ptx::ld_global(amax_in);
     const float qmax = FP8 ? 448.0f : 127.0f;
     const float scale = amax > 0.0f ? __fdiv_rn(amax, qmax) : 1.0f;
     if (blockIdx.x == 0 && threadIdx.x == 0) *scale_out = scale;
@@ -244,13 +244,13 @@ __device__ __forceinline__ uint32_t quantize_nibble(float x, const QuotientRound
 
 template <typename TIn>
 __global__ void __launch_bounds__(kQuantThreads)
-quantize_int4_kernel(const TIn* __restrict__ in, long long ld_in, uint8_t* __restrict__ out, long long ld_out_bytes,
-                     int rows, int cols, const float* __restrict__ amax_in, float* __restrict__ scale_out, int vec_ok) {
+quantize_int4_kernel(const TIn* in, long long ld_in, uint8_t* out, long long ld_out_bytes, int rows, int cols,
+                     const float* amax_in, float* scale_out, int vec_ok) {
     ptx::pdl_launch_dependents();
     ptx::pdl_wait();
     constexpr int U = Unroll<TIn>::value / 2;
     constexpr int kChunkOcts = kQuantThreads * U;
-    const float amax = __ldg(amax_in);
+    const float amax = ptx::ld_global(amax_in);
     const float scale = amax > 0.0f ? __fdiv_rn(amax, 7.0f) : 1.0f;
     if (blockIdx.x == 0 && threadIdx.x == 0) *scale_out = scale;
     const QuotientRounder qr(scale);

@@ -17,18 +17,18 @@ namespace {
 // Sums four consecutive columns over the splits (src, src + split_stride, ...) in split order and writes
 // cast(scale_a * scale_b * sum), or the raw 32-bit sum, to C[row, col .. col+3] (columns >= N left alone).
 template <bool ACC_INT>
-__device__ __forceinline__ void reduce_quad(const uint32_t* __restrict__ src, long long split_stride, int splits,
-                                            void* __restrict__ C, long long ldc, long long row, int col, int N,
-                                            int out_kind, const float* __restrict__ scale_a,
-                                            const float* __restrict__ scale_b, int c_vec_ok,
-                                            const uint32_t* __restrict__ first_src = nullptr) {
+__device__ __forceinline__ void reduce_quad(const uint32_t* src, long long split_stride, int splits, void* C,
+                                            long long ldc, long long row, int col, int N, int out_kind,
+                                            const float* scale_a, const float* scale_b, int c_vec_ok,
+                                            const uint32_t* first_src = nullptr) {
     // first_src != nullptr: term 0 is read there instead of at src (the other terms stay at src + k * split_stride)
     uint32_t raw[4];
     float f[4];
     if constexpr (ACC_INT) {
         int s[4] = {0, 0, 0, 0};
         for (int k = 0; k < splits; ++k) {
-            const uint4 v = __ldg(reinterpret_cast<const uint4*>((k == 0 && first_src != nullptr) ? first_src : src + k * split_stride));
+            const uint32_t* at = (k == 0 && first_src != nullptr) ? first_src : src + k * split_stride;
+            const uint4 v = ptx::ld_global(reinterpret_cast<const uint4*>(at));
             s[0] += static_cast<int>(v.x);
             s[1] += static_cast<int>(v.y);
             s[2] += static_cast<int>(v.z);
@@ -42,7 +42,8 @@ __device__ __forceinline__ void reduce_quad(const uint32_t* __restrict__ src, lo
     } else {
         float s[4] = {0.f, 0.f, 0.f, 0.f};
         for (int k = 0; k < splits; ++k) {
-            const uint4 v = __ldg(reinterpret_cast<const uint4*>((k == 0 && first_src != nullptr) ? first_src : src + k * split_stride));
+            const uint32_t* at = (k == 0 && first_src != nullptr) ? first_src : src + k * split_stride;
+            const uint4 v = ptx::ld_global(reinterpret_cast<const uint4*>(at));
             s[0] += __uint_as_float(v.x);
             s[1] += __uint_as_float(v.y);
             s[2] += __uint_as_float(v.z);
@@ -66,8 +67,8 @@ __device__ __forceinline__ void reduce_quad(const uint32_t* __restrict__ src, lo
         return;
     }
     float alpha = 1.0f;
-    if (scale_a != nullptr) alpha *= __ldg(scale_a);
-    if (scale_b != nullptr) alpha *= __ldg(scale_b);
+    if (scale_a != nullptr) alpha *= ptx::ld_global(scale_a);
+    if (scale_b != nullptr) alpha *= ptx::ld_global(scale_b);
 #pragma unroll
     for (int j = 0; j < 4; ++j) f[j] *= alpha;
     if (out_kind == OUT_F32) {
@@ -101,9 +102,8 @@ __device__ __forceinline__ void reduce_quad(const uint32_t* __restrict__ src, lo
 
 template <bool ACC_INT>
 __global__ void __launch_bounds__(256)
-splitk_reduce_kernel(const uint32_t* __restrict__ partials, long long split_stride, long long ldw, int splits,
-                     void* __restrict__ C, long long ldc, int M, int N, int out_kind,
-                     const float* __restrict__ scale_a, const float* __restrict__ scale_b, int c_vec_ok) {
+splitk_reduce_kernel(const uint32_t* partials, long long split_stride, long long ldw, int splits, void* C, long long ldc,
+                     int M, int N, int out_kind, const float* scale_a, const float* scale_b, int c_vec_ok) {
     ptx::pdl_launch_dependents();
     ptx::pdl_wait();
     // blockIdx.x walks along a row (four columns per thread), blockIdx.y strides over the rows: no per-thread division
@@ -119,9 +119,8 @@ splitk_reduce_kernel(const uint32_t* __restrict__ partials, long long split_stri
 // carries m_tiles, n_tiles, group_m and tile_offset, with splits = 1).
 template <bool ACC_INT>
 __global__ void __launch_bounds__(256)
-splitk_reduce_tiles_kernel(const uint32_t* __restrict__ partials, long long split_stride, int splits,
-                           void* __restrict__ C, long long ldc, int M, int N, int out_kind,
-                           const float* __restrict__ scale_a, const float* __restrict__ scale_b, int c_vec_ok,
+splitk_reduce_tiles_kernel(const uint32_t* partials, long long split_stride, int splits, void* C, long long ldc, int M,
+                           int N, int out_kind, const float* scale_a, const float* scale_b, int c_vec_ok,
                            const GemmParams tiles, int tile_n) {
     ptx::pdl_launch_dependents();
     ptx::pdl_wait();
@@ -144,9 +143,8 @@ splitk_reduce_tiles_kernel(const uint32_t* __restrict__ partials, long long spli
 // partial sums. A tile that lies in one run was stored to C by the GEMM itself.
 template <bool ACC_INT>
 __global__ void __launch_bounds__(256)
-splitk_reduce_runs_kernel(const uint32_t* __restrict__ partials, void* __restrict__ C, long long ldc, int M, int N,
-                          int out_kind, const float* __restrict__ scale_a, const float* __restrict__ scale_b,
-                          int c_vec_ok, const GemmParams tiles) {
+splitk_reduce_runs_kernel(const uint32_t* partials, void* C, long long ldc, int M, int N, int out_kind,
+                          const float* scale_a, const float* scale_b, int c_vec_ok, const GemmParams tiles) {
     ptx::pdl_launch_dependents();
     ptx::pdl_wait();
     const int tile = static_cast<int>(blockIdx.y);

@@ -75,15 +75,15 @@ __device__ __forceinline__ void transpose_block_1byte(const uint4 (&in)[16], uin
 
 template <int ES>
 __global__ void __launch_bounds__(TransposeGeom<ES>::THREADS)
-transpose_kernel(const void* __restrict__ in_v, void* __restrict__ out_v, int rows, int cols, long long ld_in,
+transpose_kernel(const void* in_v, void* out_v, int rows, int cols, long long ld_in,
                  long long ld_out, int in_vec_ok, int out_vec_ok) {
     using G = TransposeGeom<ES>;
     constexpr int B = G::B;
     constexpr int UR = G::UNITS_PER_OUT_ROW;
     __shared__ uint4 tile[G::TILE_C * UR];  // out-row c, unit u lives at c*UR + (u ^ ((c / B) % UR))
 
-    const uint8_t* __restrict__ in = reinterpret_cast<const uint8_t*>(in_v);
-    uint8_t* __restrict__ out = reinterpret_cast<uint8_t*>(out_v);
+    const uint8_t* in = reinterpret_cast<const uint8_t*>(in_v);
+    uint8_t* out = reinterpret_cast<uint8_t*>(out_v);
     const long long r0 = static_cast<long long>(blockIdx.y) * G::TILE_R;
     const long long c0 = static_cast<long long>(blockIdx.x) * G::TILE_C;
     const int tid = threadIdx.x;
@@ -100,7 +100,7 @@ transpose_kernel(const void* __restrict__ in_v, void* __restrict__ out_v, int ro
     if (in_vec_ok && gc + B <= cols && gr + B <= rows) {
 #pragma unroll
         for (int i = 0; i < B; ++i)
-            blk[i] = __ldg(reinterpret_cast<const uint4*>(in + ((gr + i) * ld_in + gc) * ES));
+            blk[i] = ptx::ld_global(reinterpret_cast<const uint4*>(in + ((gr + i) * ld_in + gc) * ES));
     } else {
 #pragma unroll
         for (int i = 0; i < B; ++i) {

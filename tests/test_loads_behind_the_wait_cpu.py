@@ -8,7 +8,6 @@ import re
 import pytest
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "qgemm_b200", "csrc")
-SOURCES = ["gemm_e8m0.cu", "gemm_e8m0.cuh", "ptx.cuh", "quantize_block.cu"]
 READ_ONLY = re.compile(r"\b__ldg\b|\b__ldcs\b|\bld\.global\.nc\b|\bconst\s+\w+\s*\*\s*__restrict__")
 
 
@@ -16,6 +15,13 @@ def code(name):
     with open(os.path.join(CSRC, name)) as f:
         text = f.read()
     return re.sub(r"//[^\n]*|/\*.*?\*/", "", text, flags=re.S)
+
+
+SOURCES = sorted(n for n in os.listdir(CSRC) if n.endswith((".cu", ".cuh")) and "pdl_" in code(n))
+
+
+def test_the_sources_are_found():
+    assert {"ptx.cuh", "gemm_launch.cuh", "quantize_block.cu", "gemm_e8m0.cuh", "splitk_reduce.cu"} <= set(SOURCES)
 
 
 @pytest.mark.parametrize("name", SOURCES)
