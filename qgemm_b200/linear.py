@@ -20,6 +20,7 @@ from contextlib import nullcontext
 from dataclasses import dataclass, field
 
 import torch
+from torch.autograd import forward_ad
 
 from . import (BLOCK, ERR_INVALID_ARG, ERR_UNSUPPORTED, QgemmError, _dtype_code, _launch, _matrix, _quantize_block,
                _scale_block_rows)
@@ -292,15 +293,23 @@ class _Fp8Linear(torch.autograd.Function):
         return dx, dw, None, None
 
 
+def _refuse_tangents(*tensors) -> None:
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise QgemmError(ERR_UNSUPPORTED, "fp8_linear has no forward-mode derivative: its input carries a tangent")
+
+
 def fp8_linear(x, weight, out_dtype=None):
     """y = x W^T in 8 bits with autograd: x [..., in] bf16 / fp16 / fp32, ``weight`` [out, in] a matrix that may require a
     gradient, or a :class:`PackedWeight` (serving; frozen layers). y has x's type unless ``out_dtype`` says otherwise.
+    Gradients are reverse-mode only: a tensor that carries a forward-mode tangent is refused, with gradients enabled or not.
     Runs on the current stream of x's device. A CUDA graph is captured after one ordinary call on the device. A leaf that the
     graph of an earlier layer call on the default stream, still alive, refers to is refused in a capture: its gradient node
     belongs to that stream, and torch would leave the capture in the backward pass. Delete what keeps that graph alive, or
     capture :func:`fp8_linear_forward` and :func:`fp8_linear_backward`, which use no autograd."""
     packed = weight if isinstance(weight, PackedWeight) else None
     w = None if packed is not None else weight
+    _refuse_tangents(x, w)
     if not torch.is_grad_enabled() or not (x.requires_grad or (w is not None and w.requires_grad)):
         return fp8_linear_forward(x, weight, False, False, out_dtype)[0]
     if not x.is_cuda:
