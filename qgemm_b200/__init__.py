@@ -351,6 +351,12 @@ def _launch(name: str, device, *args) -> None:
         raise QgemmError(rc, name)
 
 
+def _written(*tensors) -> None:
+    """Tells autograd that a caller's tensors were written to, so that a backward pass whose saved tensor was among them
+    raises an error instead of using the new values."""
+    _torch().autograd.graph.increment_version(tensors)
+
+
 def _matrix(name: str, t):
     """(rows, cols, leading dimension) of a CUDA matrix with unit inner stride whose rows do not overlap. One row has no
     leading dimension of its own: a multiple of 16, so that it asks for no alignment beyond its start's."""
@@ -461,6 +467,7 @@ def quantize_block(x, square: bool = False, form: str = "row", out=None):
         q, qld, s = _given_form(out[-2:], cols, rows, square, "column form", x.device)
         args[3:] = q.data_ptr(), qld, s.data_ptr()
     _launch("qgemm_quantize_block", x.device, _dtype_code(x), x.data_ptr(), ld, rows, cols, BLOCK if square else 1, *args)
+    _written(*out)
     return tuple(out)
 
 
@@ -476,6 +483,8 @@ def requantize_block(q, scale, out=None):
     else:
         qt, ldt, st = _given_form(out, cols, rows, False, "column form", q.device)
     _launch("qgemm_requantize_block", q.device, q.data_ptr(), ld, scale.data_ptr(), rows, cols, qt.data_ptr(), ldt, st.data_ptr())
+    if out is not None:
+        _written(qt, st)
     return qt, st
 
 
@@ -484,7 +493,8 @@ def dequantize_block(q, scale, out_dtype=None, out=None):
     torch = _torch()
     rows, cols, ld = _codes("q", q)
     block_rows = _scale_block_rows("scale", scale, rows, cols, q.device)
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty((rows, cols), dtype=out_dtype or torch.bfloat16, device=q.device)
     if out.dtype not in (torch.bfloat16, torch.float16, torch.float32):
         raise QgemmError(ERR_UNSUPPORTED, f"dequantize_block to dtype {out.dtype}")
@@ -493,6 +503,8 @@ def dequantize_block(q, scale, out_dtype=None, out=None):
         _invalid("out must have q's shape and device and the requested dtype")
     _launch("qgemm_dequantize_block", q.device, _dtype_code(out), q.data_ptr(), ld, scale.data_ptr(), block_rows, rows, cols,
             out.data_ptr(), ldo)
+    if given:
+        _written(out)
     return out
 
 
@@ -514,6 +526,7 @@ def fp8_block_mm_e8m0(a, b, a_scale, b_scale, c, accumulate: bool = False) -> No
     b_rows = _scale_block_rows("b_scale", b_scale, N, K, device)
     _launch("qgemm_fp8_block_e8m0_gemm", device, _dtype_code(c), a.data_ptr(), lda, a_scale.data_ptr(), a_rows, b.data_ptr(),
             ldb, b_scale.data_ptr(), b_rows, 1 if accumulate else 0, c.data_ptr(), ldc, M, N, K)
+    _written(c)
 
 
 MAX_DSTS = 8  # QGEMM_MAX_DSTS

@@ -23,7 +23,7 @@ import torch
 from torch.autograd import forward_ad
 
 from . import (BLOCK, ERR_INVALID_ARG, ERR_UNSUPPORTED, QgemmError, _dtype_code, _launch, _matrix, _quantize_block,
-               _scale_block_rows)
+               _scale_block_rows, _written)
 
 _TYPES = (torch.bfloat16, torch.float16, torch.float32)
 _E4M3, _E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
@@ -257,9 +257,12 @@ def fp8_linear_backward(dy, saved: LinearSaved, dw=None, accumulate: bool = Fals
         f = saved.x_form
         _launch("qgemm_requantize_block", device, kept + f.codes, f.ld, kept + f.scale, tokens, in_features,
                 base + x_across.codes, x_across.ld, base + x_across.scale)
-        if dw is None:
+        given = dw is not None
+        if not given:
             dw = torch.empty((out_features, in_features), dtype=saved.weight_dtype, device=device)
         _product(device, _at(across, base), _at(x_across, base), dw, out_features, in_features, tokens, accumulate)
+        if given:
+            _written(dw)
     return dx, dw
 
 

@@ -19,3 +19,38 @@ def test_forward_mode_tangents_are_refused(qlib, dev):
                 fp8_linear(*pair)
             assert e.value.status == qlib.ERR_UNSUPPORTED
         assert torch.equal(fp8_linear(x, w), want)
+
+
+def test_overwritten_tensors_are_noticed(qlib, dev):
+    """Every call that writes into a caller's tensor counts as a change of it in place."""
+    from qgemm_b200.linear import fp8_linear, fp8_linear_backward, fp8_linear_forward, pack_weight
+    x, w = _data(40, 256, torch.bfloat16, dev, 1), _data(40, 256, torch.float32, dev, 2)
+    q, s, qt, st = qlib.quantize_block(x, form="both")
+    back, c, dw = torch.zeros(40, 256, device=dev), torch.zeros(40, 40, device=dev), torch.zeros(40, 256, device=dev)
+    y, saved = fp8_linear_forward(x, w)
+    calls = [((q, s), lambda: qlib.quantize_block(x, out=(q, s))),
+             ((q, s, qt, st), lambda: qlib.quantize_block(x, form="both", out=(q, s, qt, st))),
+             ((qt, st), lambda: qlib.requantize_block(q, s, out=(qt, st))),
+             ((back,), lambda: qlib.dequantize_block(q, s, out=back)),
+             ((c,), lambda: qlib.fp8_block_mm_e8m0(q, q, s, s, c)),
+             ((c,), lambda: qlib.fp8_block_mm_e8m0(q, q, s, s, c, accumulate=True)),
+             ((dw,), lambda: fp8_linear_backward(y, saved, dw=dw)),
+             ((dw,), lambda: fp8_linear_backward(y, saved, dw=dw, accumulate=True))]
+    for tensors, call in calls:
+        before = [t._version for t in tensors]
+        call()
+        assert all(t._version > b for t, b in zip(tensors, before))
+    with torch.inference_mode():
+        qlib.dequantize_block(q, s, out=back)
+        qlib.dequantize_block(q, s, out=torch.zeros(40, 256, device=dev))  # a tensor without a version
+    p = torch.ones(40, 256, device=dev, requires_grad=True)
+    z = (p * back).sum()  # keeps `back` for p's gradient
+    qlib.dequantize_block(q, s, out=back)
+    with pytest.raises(RuntimeError):
+        z.backward()
+    packed = pack_weight(w, backward=True)
+    xi = x.clone().requires_grad_(True)
+    y = fp8_linear(xi, packed)
+    qlib.quantize_block(w, square=True, form="both", out=(packed.codes, packed.scale, packed.codes_t, packed.scale_t))
+    with pytest.raises(RuntimeError):
+        y.sum().backward()
