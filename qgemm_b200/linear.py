@@ -275,6 +275,20 @@ def _accumulators(*leaves):
             if t is not None and t.requires_grad and t.is_leaf]
 
 
+def _as_saved(buffer, weight_t):
+    """A saved buffer and transposed weight as the kernels take them. Saved-tensor hooks (offloading to the host) give back
+    equal tensors, but at any address and without the padding that starts a weight's rows on 16-byte boundaries."""
+    if buffer is not None and (buffer.data_ptr() % 16 or not buffer.is_contiguous()):
+        buffer = buffer.clone(memory_format=torch.contiguous_format)
+    if not weight_t:
+        return buffer, None
+    codes, scale = weight_t
+    rows, cols = codes.shape
+    if codes.data_ptr() % 16 or codes.stride(0) % 16 or codes.stride(1) != 1:
+        codes = torch.empty_strided((rows, cols), ((cols + 15) & -16, 1), dtype=codes.dtype, device=codes.device).copy_(codes)
+    return buffer, (codes, scale.contiguous())
+
+
 class _Fp8Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, packed, out_dtype):
@@ -290,8 +304,9 @@ class _Fp8Linear(torch.autograd.Function):
     def backward(ctx, dy):
         r = ctx.rest
         buffer, *weight_t = ctx.saved_tensors
-        saved = LinearSaved(buffer, r.x_form, r.weight_form, tuple(weight_t) or None, r.x_shape, r.x_dtype, r.weight_dtype,
-                            r.out_features, r.device)
+        buffer, weight_t = _as_saved(buffer, weight_t)
+        saved = LinearSaved(buffer, r.x_form, r.weight_form, weight_t, r.x_shape, r.x_dtype, r.weight_dtype, r.out_features,
+                            r.device)
         dx, dw = fp8_linear_backward(dy, saved)
         return dx, dw, None, None
 

@@ -19,3 +19,19 @@ def test_forward_mode_tangents_are_refused(qlib, of, grad):
         with pytest.raises(qlib.QgemmError) as e:
             fp8_linear(x, w)
     assert e.value.status == qlib.ERR_UNSUPPORTED
+
+
+def test_saved_tensors_come_back_as_the_kernels_take_them():
+    from qgemm_b200.linear import _as_saved
+    g = torch.Generator().manual_seed(1)
+    codes = torch.randint(0, 120, (130, 77), generator=g, dtype=torch.uint8).view(torch.float8_e4m3fn)  # padding lost
+    scale = torch.randint(0, 255, (2, 1), generator=g, dtype=torch.uint8).view(torch.float8_e8m0fnu).t()
+    wide = torch.randint(0, 255, (1000,), generator=g, dtype=torch.uint8)
+    moved = wide[3 - wide.data_ptr() % 16:][:900]  # 3 bytes past a boundary
+    buffer, (c, s) = _as_saved(moved, (codes, scale))
+    assert buffer.data_ptr() % 16 == 0 and torch.equal(buffer, moved)
+    assert c.data_ptr() % 16 == 0 and c.stride() == (80, 1) and torch.equal(c.view(torch.uint8), codes.view(torch.uint8))
+    assert s.is_contiguous() and torch.equal(s.view(torch.uint8), scale.view(torch.uint8))
+    for kept in (_as_saved(buffer, (c, s)), _as_saved(buffer, ())):  # what fits is not copied
+        assert kept[0] is buffer and (kept[1] is None or kept[1][0] is c)
+    assert _as_saved(None, None) == (None, None)

@@ -54,3 +54,51 @@ def test_overwritten_tensors_are_noticed(qlib, dev):
     qlib.quantize_block(w, square=True, form="both", out=(packed.codes, packed.scale, packed.codes_t, packed.scale_t))
     with pytest.raises(RuntimeError):
         y.sum().backward()
+
+
+def _unaligned(t):
+    """An equal tensor three bytes past a boundary, without the original's padding."""
+    buf = torch.empty(t.numel() * t.element_size() + 16, dtype=torch.uint8, device=t.device)
+    flat = buf[3:3 + t.numel() * t.element_size()]
+    flat.copy_(t.contiguous().view(-1).view(torch.uint8))
+    return flat.view(t.dtype).view(t.shape)
+
+
+@pytest.mark.parametrize("out_features", [128, 130])
+@pytest.mark.parametrize("packed", [False, True])
+def test_saved_tensor_hooks(qlib, dev, out_features, packed):
+    """Saved tensors kept on the host, or anywhere else on the device, until the backward pass."""
+    from qgemm_b200.linear import fp8_linear, pack_weight
+    x, w = _data(33, 200, torch.bfloat16, dev, 1), _data(out_features, 200, torch.float32, dev, 2)
+    dy = _data(33, out_features, torch.bfloat16, dev, 3)
+
+    def gradients():
+        xi, wi = x.clone().requires_grad_(True), w.clone().requires_grad_(not packed)
+        y = fp8_linear(xi, pack_weight(wi, backward=True) if packed else wi)
+        return xi, wi, y
+
+    xi, wi, y = gradients()
+    y.backward(dy)
+    want = (xi.grad, wi.grad)
+    for hooks in (torch.autograd.graph.save_on_cpu(), torch.autograd.graph.save_on_cpu(pin_memory=True),
+                  torch.autograd.graph.saved_tensors_hooks(_unaligned, lambda t: t)):
+        with hooks:
+            xi, wi, y = gradients()
+        y.backward(dy)
+        assert torch.equal(xi.grad, want[0])
+        assert packed or torch.equal(wi.grad, want[1])
+
+
+def test_recomputed_in_the_backward_pass(qlib, dev):
+    from torch.utils.checkpoint import checkpoint
+
+    from qgemm_b200.linear import fp8_linear
+    x, w = _data(33, 200, torch.bfloat16, dev, 1), _data(130, 200, torch.float32, dev, 2)
+    got = []
+    for again in (False, True):
+        xi, wi = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        y = checkpoint(fp8_linear, xi, wi, use_reentrant=False) if again else fp8_linear(xi, wi)
+        y.square().sum().backward()
+        got.append((y.detach(), xi.grad, wi.grad))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
