@@ -82,6 +82,7 @@ class LinearSaved:
     weight_dtype: torch.dtype | None
     out_features: int
     device: torch.device = field(default=None)
+    stream: int = 0  # the forward call's, to which the buffer's memory belongs
 
     @property
     def x(self):
@@ -204,14 +205,16 @@ def fp8_linear_forward(x, weight, need_dx: bool = True, need_dw: bool = True, ou
     _product(device, _at(x_form, x_base), w_at, y, tokens, out_features, in_features)
     saved = LinearSaved(buffer, x_form if need_dw else None, wt_form,
                         (weight.codes_t, weight.scale_t) if packed and need_dx else None, tuple(x.shape), x.dtype,
-                        None if packed else weight.dtype, out_features, device)
+                        None if packed else weight.dtype, out_features, device,
+                        torch._C._cuda_getCurrentRawStream(device.index))
     return (y if x.dim() == 2 else y.view(*x.shape[:-1], out_features)), saved
 
 
 def fp8_linear_backward(dy, saved: LinearSaved, dw=None, accumulate: bool = False):
     """``(dx, dw)`` from dy [..., out] and what the forward call saved; None for a gradient it saved nothing for. ``dw``: a
     matrix [out, in] to write into instead of a new one, or with ``accumulate`` (fp32) to add to, as over the micro-batches
-    of one step."""
+    of one step. It may run on another stream than the forward call, once that stream waits for it; ``saved`` may then be
+    dropped at once."""
     out_features, in_features = saved.out_features, saved.x_shape[-1]
     dy2 = _flat(dy, out_features, "dy")
     device = saved.device
@@ -244,7 +247,12 @@ def fp8_linear_backward(dy, saved: LinearSaved, dw=None, accumulate: bool = Fals
         at = x_across.end
     scratch = torch.empty(at, dtype=torch.uint8, device=device)
     base = scratch.data_ptr()
-    kept = saved.buffer.data_ptr() if saved.buffer is not None else 0
+    kept = 0
+    if saved.buffer is not None:
+        kept = saved.buffer.data_ptr()
+        if torch._C._cuda_getCurrentRawStream(device.index) != saved.stream:
+            # nobody else knows of this use: without it the memory could be given out again before these kernels are done
+            saved.buffer.record_stream(torch.cuda.current_stream(device))
     _quantize(device, dy2, base, along, across)
     dx = None
     if need_dx:
@@ -306,7 +314,7 @@ class _Fp8Linear(torch.autograd.Function):
         buffer, *weight_t = ctx.saved_tensors
         buffer, weight_t = _as_saved(buffer, weight_t)
         saved = LinearSaved(buffer, r.x_form, r.weight_form, weight_t, r.x_shape, r.x_dtype, r.weight_dtype, r.out_features,
-                            r.device)
+                            r.device, r.stream)
         dx, dw = fp8_linear_backward(dy, saved)
         return dx, dw, None, None
 

@@ -102,3 +102,29 @@ def test_recomputed_in_the_backward_pass(qlib, dev):
         got.append((y.detach(), xi.grad, wi.grad))
     for a, b in zip(*got):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("need_dx,need_dw", [(True, True), (False, True), (True, False)])
+def test_backward_on_another_stream_keeps_what_was_saved(qlib, dev, need_dx, need_dw):
+    """The backward pass is queued behind a delay on a second stream and `saved` dropped at once: the forward's stream, which
+    takes memory and writes to it meanwhile, must not be given the saved codes' memory."""
+    from qgemm_b200.linear import fp8_linear_backward, fp8_linear_forward
+    x, w = _data(300, 1024, torch.bfloat16, dev, 1), _data(900, 1024, torch.bfloat16, dev, 2)
+    dy = _data(300, 900, torch.bfloat16, dev, 3)
+    want = fp8_linear_backward(dy, fp8_linear_forward(x, w, need_dx, need_dw)[1])
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(one):
+        saved = fp8_linear_forward(x, w, need_dx, need_dw)[1]
+        size = saved.buffer.numel()
+    two.wait_stream(one)
+    with torch.cuda.stream(two):
+        torch.cuda._sleep(100_000_000)  # about 50 ms
+        got = fp8_linear_backward(dy, saved)
+    del saved
+    with torch.cuda.stream(one):
+        others = [torch.full((size,), 0x7F, dtype=torch.uint8, device=dev) for _ in range(4)]
+    torch.cuda.synchronize()
+    for g, r in zip(got, want):
+        assert (g is None and r is None) or torch.equal(g, r)
+    del others
