@@ -274,13 +274,56 @@ def fp8_linear_backward(dy, saved: LinearSaved, dw=None, accumulate: bool = Fals
     return dx, dw
 
 
-_DEFAULT_STREAM = "qgemm_b200.linear: made on the default stream"
+# Where the gradient of a leaf is gathered: its node belongs to the stream that was current when the node was made, and lives
+# as long as any graph refers to the leaf. torch does not tell the stream, so the layer's calls write it into the node.
+_STREAM = "qgemm_b200.linear: stream"
+_PROBE = "qgemm_b200.linear: probe"
 
 
-def _accumulators(*leaves):
-    """The nodes that end a graph at those of the tensors that are leaves with a gradient."""
-    return [torch.autograd.graph.get_gradient_edge(t).node for t in leaves
-            if t is not None and t.requires_grad and t.is_leaf]
+def _leaf_node(node):
+    """The leaf's node that ``node`` leads to by way of at most four operations of one input each (casts, transposes), or
+    None. A leaf's node is its own."""
+    for _ in range(5):
+        following = node.next_functions
+        if not following and hasattr(node, "variable"):
+            return node
+        if len(following) != 1 or following[0][0] is None:
+            return None
+        node = following[0][0]
+    return None
+
+
+def _node(t):
+    """The node that gathers or passes on t's gradient."""
+    return t.view_as(t).grad_fn.next_functions[0][0] if t.is_leaf else t.grad_fn
+
+
+def _probe_nodes(capturing: bool, *tensors) -> None:
+    """Before a call on a stream other than the default one: refuses a capture whose backward pass would come to a node of
+    the default stream, and writes into the nodes that live already that they do."""
+    for t in tensors:
+        if t is None or not t.requires_grad:
+            continue
+        # through a derived tensor's graph a node lives in any case: only a refusal looks there
+        node = _node(t) if t.is_leaf else (_leaf_node(t.grad_fn) if capturing else None)
+        if node is None:
+            continue
+        if capturing and node.metadata.get(_STREAM) == 0:
+            del node  # the error's traceback must not keep it alive
+            raise QgemmError(ERR_UNSUPPORTED, "capturing a graph while an earlier graph of the same leaves is alive")
+        node.metadata[_PROBE] = True  # gone with the last reference to the node, here if no graph holds one
+
+
+def _note_nodes(y, stream: int) -> None:
+    """After a call: the nodes it made are its stream's. One that lived before and has no mark counts as the default stream's
+    once a call there has met it."""
+    for node, _ in y.grad_fn.next_functions:
+        if node is not None and node.next_functions:
+            node = _leaf_node(node) if stream == 0 else None
+        if node is None:
+            continue
+        if stream == 0 or _PROBE not in node.metadata:
+            node.metadata.setdefault(_STREAM, stream)
 
 
 def _as_saved(buffer, weight_t):
@@ -329,10 +372,15 @@ def fp8_linear(x, weight, out_dtype=None):
     """y = x W^T in 8 bits with autograd: x [..., in] bf16 / fp16 / fp32, ``weight`` [out, in] a matrix that may require a
     gradient, or a :class:`PackedWeight` (serving; frozen layers). y has x's type unless ``out_dtype`` says otherwise.
     Gradients are reverse-mode only: a tensor that carries a forward-mode tangent is refused, with gradients enabled or not.
-    Runs on the current stream of x's device. A CUDA graph is captured after one ordinary call on the device. A leaf that the
-    graph of an earlier layer call on the default stream, still alive, refers to is refused in a capture: its gradient node
-    belongs to that stream, and torch would leave the capture in the backward pass. Delete what keeps that graph alive, or
-    capture :func:`fp8_linear_forward` and :func:`fp8_linear_backward`, which use no autograd."""
+    Runs on the current stream of x's device. A CUDA graph is captured after one ordinary call on the device.
+
+    A capture is refused while an earlier graph of the same leaves, made on the default stream, is alive: the leaves' gradient
+    nodes then belong to that stream, and torch would leave the capture in the backward pass. The refusal sees x and the
+    weight themselves, or their leaves through up to four one-input operations (casts, transposes), where an earlier call of
+    this function on the default stream met them; a leaf that only other operations used there is not seen. (A node that
+    other operations made on some other stream and a default-stream call of this function met counts as the default
+    stream's.) Delete what keeps that graph alive, or capture :func:`fp8_linear_forward` and :func:`fp8_linear_backward`,
+    which use no autograd."""
     packed = weight if isinstance(weight, PackedWeight) else None
     w = None if packed is not None else weight
     _refuse_tangents(x, w)
@@ -341,13 +389,10 @@ def fp8_linear(x, weight, out_dtype=None):
     if not x.is_cuda:
         raise QgemmError(ERR_INVALID_ARG, "x must be a CUDA tensor (there is no CPU path)")
     stream = torch.cuda.current_stream(x.device).cuda_stream
-    if stream != 0:  # the default stream is never captured, and no other's graph hinders a capture
+    if stream != 0:  # the default stream is never captured
         with nullcontext() if torch.cuda.current_device() == x.device.index else torch.cuda.device(x.device):
             capturing = torch.cuda.is_current_stream_capturing()
-        if capturing and any(n.metadata.get(_DEFAULT_STREAM) for n in _accumulators(x, w)):
-            raise QgemmError(ERR_UNSUPPORTED, "capturing a graph while an earlier graph of the same leaves is alive")
+        _probe_nodes(capturing, x, w)
     y = _Fp8Linear.apply(x, w, packed, out_dtype)
-    if stream == 0:
-        for node in _accumulators(x, w):  # alive as long as a graph refers to the leaf, and its mark with it
-            node.metadata[_DEFAULT_STREAM] = True
+    _note_nodes(y, stream)
     return y

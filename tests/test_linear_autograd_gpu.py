@@ -128,3 +128,42 @@ def test_backward_on_another_stream_keeps_what_was_saved(qlib, dev, need_dx, nee
     for g, r in zip(got, want):
         assert (g is None and r is None) or torch.equal(g, r)
     del others
+
+
+@pytest.mark.parametrize("weight", ["cast", "transposed"])
+def test_capture_beside_a_living_graph_of_a_derived_weight_is_refused(qlib, dev, weight):
+    from qgemm_b200.linear import fp8_linear
+    x = _data(20, 64, torch.bfloat16, dev, 1)
+    w = _data(64, 64, torch.float32, dev, 2).requires_grad_(True)
+    derive = {"cast": lambda: w.to(torch.bfloat16), "transposed": lambda: w.t()}[weight]
+    alive = fp8_linear(x, derive())
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(qlib.QgemmError) as e:
+        with torch.cuda.graph(graph):
+            fp8_linear(x, w)
+    assert e.value.status == qlib.ERR_UNSUPPORTED
+    alive.sum().backward()
+    assert w.grad.shape == w.shape
+
+
+def test_capture_beside_a_side_streams_graph_that_the_default_stream_used_too(qlib, dev):
+    """The leaf's node was made by a call on a side stream and is still alive; a later call on the default stream does not
+    make it that one's."""
+    from qgemm_b200.linear import fp8_linear
+    x = _data(20, 256, torch.bfloat16, dev, 1)
+    w = _data(40, 256, torch.float32, dev, 2).requires_grad_(True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        alive = fp8_linear(x, w)
+    torch.cuda.current_stream().wait_stream(side)
+    want, = torch.autograd.grad(fp8_linear(x, w).sum(), w)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got, = torch.autograd.grad(fp8_linear(x, w).sum(), w)
+    got.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    del alive
