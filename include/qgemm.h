@@ -252,7 +252,8 @@ int qgemm_device_status(int* out4);
  * QGEMM_GROUP_M, QGEMM_CTA_PAIR, QGEMM_RELAYOUT_B, QGEMM_MAX_CTAS, QGEMM_DIRECT_STORE, QGEMM_FULL_A_TILE,
  * QGEMM_TAIL_SPLIT, QGEMM_BALANCE, QGEMM_PREFETCH, QGEMM_KCLUSTER, QGEMM_KGROUP, QGEMM_EARLY_GROUPS, QGEMM_ONE_TILE, QGEMM_EVEN_RUNS, QGEMM_E8M0_TILE_M, QGEMM_E8M0_TILE_N, QGEMM_E8M0_SLICES, QGEMM_HOST_BANDS, QGEMM_HOST_BANDS_N) are
  * read once, when the library is
- * loaded; this reads them again. Not meant to run concurrently with GEMM calls of other threads.
+ * loaded; this reads them again. Not meant to run concurrently with GEMM calls of other threads. QGEMM_E8M0_* settings that
+ * no form of the block-scaled product has, or none that suits a call's K, are set aside for that call.
  */
 int qgemm_reload_env(void);
 

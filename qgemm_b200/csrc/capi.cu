@@ -994,15 +994,19 @@ E8m0Plan plan_e8m0(size_t M, size_t N, size_t K, int sms) {
     const int kb = static_cast<int>((K + 127) / 128);
     E8m0Plan best = kForms[0];
     double best_us = 1e30;
-    for (const E8m0Plan& f : kForms) {
-        if (f.slices > kb) continue;
-        if ((g_env.e8m0_tile_m > 0 && f.tile_m != g_env.e8m0_tile_m) || (g_env.e8m0_tile_n > 0 && f.tile_n != g_env.e8m0_tile_n) ||
-            (g_env.e8m0_slices > 0 && f.slices != g_env.e8m0_slices))
-            continue;
-        const double us = estimate_e8m0(f, M, N, K, sms);
-        if (us < best_us) {
-            best = f;
-            best_us = us;
+    // among the forms that the settings ask for, or, when none of those exists or suits this K, among all
+    for (int asked = 1; asked >= 0 && best_us == 1e30; --asked) {
+        for (const E8m0Plan& f : kForms) {
+            if (f.slices > kb) continue;
+            if (asked != 0 && ((g_env.e8m0_tile_m > 0 && f.tile_m != g_env.e8m0_tile_m) ||
+                               (g_env.e8m0_tile_n > 0 && f.tile_n != g_env.e8m0_tile_n) ||
+                               (g_env.e8m0_slices > 0 && f.slices != g_env.e8m0_slices)))
+                continue;
+            const double us = estimate_e8m0(f, M, N, K, sms);
+            if (us < best_us) {
+                best = f;
+                best_us = us;
+            }
         }
     }
     return best;

@@ -28,3 +28,29 @@ def test_operands_rewritten_between_calls(qlib, dev, M, N, K):
     for i, outs in enumerate(got):
         for g, r in zip(outs, want[i % 3]):
             assert torch.equal(g, r), i
+
+
+@pytest.mark.parametrize("K,settings", [(4096, {"TILE_M": 48}), (4096, {"TILE_M": 64, "TILE_N": 256}), (4096, {"SLICES": 3}),
+                                        (896, {"SLICES": 8})])
+def test_settings_that_no_form_has_are_set_aside(qlib, dev, monkeypatch, K, settings):
+    """The call then takes the form it would have taken without them, recognised by the order of its fp32 sums."""
+    a, sa = qlib.quantize_block(_data(64, K, torch.float32, dev, 1))
+    b, sb = qlib.quantize_block(_data(520, K, torch.float32, dev, 2))
+
+    def product(**env):
+        for name in ("TILE_M", "TILE_N", "SLICES"):
+            monkeypatch.delenv("QGEMM_E8M0_" + name, raising=False)
+        for name, value in env.items():
+            monkeypatch.setenv("QGEMM_E8M0_" + name, str(value))
+        qlib.lib().qgemm_reload_env()
+        c = torch.empty(64, 520, device=dev)
+        qlib.fp8_block_mm_e8m0(a, b, sa, sb, c)
+        return c
+
+    try:
+        free, one_slice = product(), product(TILE_M=16, SLICES=1)
+        assert not torch.equal(free, one_slice)  # or the comparison would show nothing
+        assert torch.equal(product(**settings), free)
+    finally:
+        monkeypatch.undo()
+        qlib.lib().qgemm_reload_env()
