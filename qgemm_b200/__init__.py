@@ -512,8 +512,12 @@ def fp8_block_mm_e8m0(a, b, a_scale, b_scale, c, accumulate: bool = False) -> No
     """c[m,n] = a[m,k] x b[n,k]^T of FP8 codes with power-of-two block scales (:func:`quantize_block`), the scales applied
     by the tensor cores; argument order as :func:`fp8_block_mm`. ``a_scale`` [ceil(k/128), m] or, one for 128 rows,
     [ceil(k/128), ceil(m/128)]; ``b_scale`` likewise of n. ``c`` bf16 / fp16 / fp32; ``accumulate`` adds to what a fp32 ``c``
-    holds (numbers below 2^-126 count as zeros there). Rows of ``a`` and ``b`` start on 16-byte boundaries. A layer's three products, with x, w and dy quantised:
-    forward (x row, w row), dx = (dy row, w column), dw = (dy column, x column)."""
+    holds (numbers below 2^-126 count as zeros there). Rows of ``a`` and ``b`` start on 16-byte boundaries. A layer's three
+    products, with x, w and dy quantised: forward (x row, w row), dx = (dy row, w column), dw = (dy column, x column).
+
+    The tensor cores' sums are cut off, not rounded: an element of a fp32 ``c`` is within 2.2e-4 * sum |a b| of the exact one
+    for any k, reached only where the first of k outweigh all the rest; the error's norm is about 3e-7 of c's for values of
+    random sign and 2e-6 for values of one sign (``qgemm.h``)."""
     M, K, lda = _codes("a", a)
     N, Kb, ldb = _codes("b", b)
     rows, cols, ldc = _matrix("c", c)

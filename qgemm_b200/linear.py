@@ -9,7 +9,8 @@ With Q the quantisation to FP8 e4m3 over blocks of 128 along the axis a product 
 
 What the forward pass saves of x is Q(x), one byte an element plus 1/128: the codes its own product read. The backward pass
 makes the operand of dW from them, quantised anew along the tokens (:func:`qgemm_b200.requantize_block`), so training keeps
-no 16- or 32-bit copy of the activation. All sums are fp32; y, dx have x's type and dW has W's, each rounded once.
+no 16- or 32-bit copy of the activation. All sums are fp32, made as :func:`qgemm_b200.fp8_block_mm_e8m0` says; y, dx have
+x's type and dW has W's, each rounded once.
 
 Gradients pass through Q as through the identity. The reference has no layer and no backward pass; its ``fp8_mm(a, b, as, bs,
 c)`` (src/mix_gemm/hip_mix_gemm_kernel.cpp:508-516) is the forward product alone.

@@ -1,0 +1,70 @@
+"""How far sums of the block-scaled product may be off in fp32, element by element, where the truncation of the tensor cores'
+additions tells most: sums of one sign, and a first block that outweighs all the rest.
+
+Bound, for each 32 of K: 32 products and the running sum are cut to multiples of 2^-25 of the largest one's power of two,
+which is at most S = sum |a b|, and the new sum to 24 bits: (33 / 4 + 1) steps of 2^-23 S. A chain has at most 48 K blocks, 192
+such additions; the chains' losses add up to no more than that many steps of the whole S. Joining 8 slices and P parts, and
+adding to what C held, is one rounding each of at most S + |C|: half a step."""
+import math
+
+import pytest
+import torch
+
+from block_reference import E4M3, E8M0, values
+from test_block_e8m0_gpu import _data
+
+pytestmark = pytest.mark.gpu
+
+STEP = 2.0 ** -23
+
+
+def _bound(K, mags):
+    chain = min(math.ceil(K / 32), 192)
+    parts = math.ceil(K / 6144) + 1
+    return (9.25 * chain + 0.5 * (8 + parts)) * STEP * mags
+
+
+def _check(qlib, a, sa, b, sb, accumulate):
+    av, bv = values(a, sa).to(a.device), values(b, sb).to(a.device)
+    ref, mags = av @ bv.t(), av.abs() @ bv.abs().t()
+    c = torch.zeros(ref.shape, device=a.device)
+    if accumulate:
+        c = torch.randn(ref.shape, device=a.device) * float(ref.abs().mean())
+        ref, mags = ref + c.double(), mags + c.double().abs()
+    K = a.shape[1]
+    qlib.fp8_block_mm_e8m0(a, b, sa, sb, c, accumulate=accumulate)
+    assert float(((c.double() - ref).abs() - _bound(K, mags)).max()) <= 0
+    return c, ref
+
+
+SHAPES = [(16, 512, 65536), (70, 200, 6145), (300, 520, 16500), (1100, 2100, 12300)]
+
+
+@pytest.mark.parametrize("M,N,K", SHAPES)
+@pytest.mark.parametrize("one_sign", [False, True])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_first_block_outweighs_the_rest(qlib, dev, M, N, K, one_sign, accumulate):
+    x, w = _data(M, K, torch.float32, dev, 1, 0.5), _data(N, K, torch.float32, dev, 2, 0.5)
+    if one_sign:
+        x, w = x.abs(), w.abs()
+    x[:, :256] *= 1024.0
+    a, sa = qlib.quantize_block(x)
+    b, sb = qlib.quantize_block(w)
+    _check(qlib, a, sa, b, sb, accumulate)
+
+
+@pytest.mark.parametrize("M,N,K", SHAPES)
+@pytest.mark.parametrize("below", [24, 25, 26, 27])
+def test_products_at_the_running_sums_last_bits(qlib, dev, M, N, K, below):
+    """A 1, then products of 15/8 * 2^-below: what is lost of each is the largest part there is."""
+    kb = -(-K // 128)
+    ld = -(-K // 16) * 16
+    a = torch.zeros(M, ld, dtype=torch.uint8, device=dev)
+    b = torch.full((N, ld), 0x38, dtype=torch.uint8, device=dev)  # 1
+    a[:, 0] = 0x38
+    a[:, 128:K] = 0x3F  # 15/8
+    sa = torch.full((kb, M), 127 - below, dtype=torch.uint8, device=dev)
+    sa[0] = 127
+    sb = torch.full((kb, N), 127, dtype=torch.uint8, device=dev)
+    c, ref = _check(qlib, a.view(E4M3)[:, :K], sa.view(E8M0), b.view(E4M3)[:, :K], sb.view(E8M0), False)
+    assert bool((c <= ref.float()).all()) and bool((c >= 1).all())  # cut off towards zero, never below what is there
