@@ -174,7 +174,8 @@ int qgemm_dequantize_block(int out_dtype, const void* q, size_t ld_q, const void
  * so that an element's error stays below 2.2e-4 * sum |a b| however long K is. That bound is for a first block that
  * outweighs all the rest; norm of the error over the norm of C as measured at 2304 x 2048, K = 6144 / 16384: values of
  * random sign 3.5e-7 / 3.1e-7, of one sign 2.5e-6 / 2.1e-6, of one sign with the first 256 of K a thousandfold 2.3e-5 /
- * 1.9e-5.
+ * 1.9e-5. Those additions too take numbers below 2^-126 as zeros: an FP32 result that small is exact up to K = 6144, and
+ * beyond may be a zero, whether accumulate is set or not.
  * Any M, N, K >= 0 (K = 0: zeros, or C unchanged when accumulating). No library scratch is used, so calls on several
  * streams are independent; results are reproducible. The first GEMM call on a device must not be inside a stream capture.
  */

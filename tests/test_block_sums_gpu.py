@@ -68,3 +68,34 @@ def test_products_at_the_running_sums_last_bits(qlib, dev, M, N, K, below):
     sb = torch.full((kb, N), 127, dtype=torch.uint8, device=dev)
     c, ref = _check(qlib, a.view(E4M3)[:, :K], sa.view(E8M0), b.view(E4M3)[:, :K], sb.view(E8M0), False)
     assert bool((c <= ref.float()).all()) and bool((c >= 1).all())  # cut off towards zero, never below what is there
+
+
+@pytest.mark.parametrize("M,N,K,several", [(16, 128, 6144, False), (300, 512, 6100, False), (2304, 2176, 6144, False),
+                                           (2301, 2175, 640, False), (16, 128, 70000, True), (16, 127, 50000, True),
+                                           (2304, 2176, 6200, None), (2301, 2175, 6200, None), (300, 512, 16500, None)])
+@pytest.mark.parametrize("at", ["first", "last"])
+def test_results_below_the_normal_numbers(qlib, dev, M, N, K, several, at):
+    """One product an element, between 2^-131 and 2^-121. Exact in one launch, which every form makes up to K = 6144; zeros
+    below 2^-126 in several, which every form makes beyond 8 slices of 6144; one or the other in between."""
+    kb, ld = -(-K // 128), -(-K // 16) * 16
+    a, b = (torch.zeros(n, ld, dtype=torch.uint8, device=dev) for n in (M, N))
+    k = 0 if at == "first" else K - 1
+    a[:, k] = 0x38  # 1
+    b[:, k] = torch.tensor([0x38, 0x3C, 0xB8, 0x30], dtype=torch.uint8, device=dev)[torch.arange(N, device=dev) % 4]
+    sa = (torch.arange(M, device=dev) % 8 + 60).to(torch.uint8).expand(kb, M).contiguous()
+    sb = torch.full((kb, N), 64, dtype=torch.uint8, device=dev)
+    c = torch.full((M, N), 7.0, device=dev)
+    qlib.fp8_block_mm_e8m0(a.view(E4M3)[:, :K], b.view(E4M3)[:, :K], sa.view(E8M0), sb.view(E8M0), c)
+    lo = k // 128 * 128
+    ref = (values(a.view(E4M3)[:, lo:min(lo + 128, K)], sa[lo // 128:lo // 128 + 1])
+           @ values(b.view(E4M3)[:, lo:min(lo + 128, K)], sb[lo // 128:lo // 128 + 1]).t()).to(dev)
+    small = ref.abs() < 2.0 ** -126
+    assert bool(small.any()) and not bool(small.all())
+    exact = c.double() == ref
+    assert bool(exact[~small].all())
+    if several is False:
+        assert bool(exact.all())
+    elif several:
+        assert bool((c[small] == 0).all())
+    else:
+        assert bool((exact | (c == 0)).all())
