@@ -1122,6 +1122,7 @@ int e8m0_launch(const E8m0Plan& plan, const void* A, size_t lda, const void* B, 
     std::memset(&tc, 0, sizeof(tc));
     if (c_addr % 16 == 0 && (static_cast<size_t>(p.ldc) * out_bytes) % 16 == 0 && g_env.direct_store == 0)
         p.c_tma_ok = encode_output_map(p.C, p.M, p.N, p.ldc, 1, p.out, &tc) == QGEMM_OK ? 1 : 0;
+    p.n_tma = tma_store_columns(p.N, static_cast<int>(out_bytes));
     // tile rows walked together, so that their panels of A (16 MB of them) stay in L2 while B passes
     p.group_m = static_cast<int>(std::max<long long>(4, (16ll << 20) / (128ll * p.kb_total * 256)));
     p.group_m = std::min(g_env.group_m > 0 ? g_env.group_m : p.group_m, p.m_tiles);

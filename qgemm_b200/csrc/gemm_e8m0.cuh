@@ -37,6 +37,7 @@ struct E8m0Params {
     int out;               // OUT_F32 / OUT_BF16 / OUT_F16
     int accumulate;        // fp32 C: add to what it holds
     int c_tma_ok, c_vec_ok;
+    int n_tma;         // boxes of C that begin before this column are stored by TMA (tma_store_columns)
     int test_skip_kb;  // failure-detection test hook: the producers leave out this K block (-1 = none)
     int* status;
 };
@@ -549,12 +550,12 @@ struct E8PairSmem {
     static_assert(kAccStep + BN <= kScaleCol && kScaleCol + kE8Cols * kScaleCols <= 512, "tensor-memory columns");
 };
 
-// A staged box to a C that TMA cannot address (any ldc, any base aligned to its element): a warp writes a row's 128 bytes
-// at a time; 16-bit rows as words where the row starts on one. fp32 rows are read from the box eight at a time before the
-// first of them is written, and an accumulating product adds without reading C: row after row 8192 x 4096 x 4096 took 126 us
-// instead of 106, and 890 instead of 110 accumulating. (16-bit rows gain nothing by eights; rows that start inside a word,
-// shifted between the lanes and stored as words, took 164 us there instead of 95. From registers, a row a lane,
-// 2500 x 2500 x 8192 took 115 us.)
+// A staged box to a C that TMA cannot address (any ldc, any base aligned to its element), or to the last columns of one that
+// do not end on 16 bytes: a warp writes a row's 128 bytes at a time; 16-bit rows as words where the row starts on one. fp32
+// rows are read from the box eight at a time before the first of them is written, and an accumulating product adds without
+// reading C: row after row 8192 x 4096 x 4096 took 126 us instead of 106, and 890 instead of 110 accumulating. (16-bit rows
+// gain nothing by eights; rows that start inside a word, shifted between the lanes and stored as words, took 164 us there
+// instead of 95. From registers, a row a lane, 2500 x 2500 x 8192 took 115 us.)
 template <int OUT>
 __device__ __forceinline__ void store_box_rows(const E8m0Params& p, uint32_t box, int row0, int n0, int lane) {
     constexpr int OB = OutBytes<OUT>::value;
@@ -819,6 +820,7 @@ gemm_e8m0_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
                     }
                 }
                 // a staged box of 32 rows x 128 bytes; it is free once the store before has read it
+                const bool by_tma = p.c_tma_ok && n0 < p.n_tma;
                 if (p.c_tma_ok && ptx::elect_one()) ptx::tma_store_wait_read<0>();
                 __syncwarp();
                 const uint32_t row_addr = stage_base + static_cast<uint32_t>(lane) * 128u;
@@ -826,7 +828,7 @@ gemm_e8m0_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
                 for (int j = 0; j < 8; ++j)
                     ptx::st_shared_v4(row_addr + static_cast<uint32_t>((j ^ (lane & 7)) * 16), u[4 * j], u[4 * j + 1],
                                       u[4 * j + 2], u[4 * j + 3]);
-                if (p.c_tma_ok) {
+                if (by_tma) {
                     ptx::fence_proxy_async_smem();
                     __syncwarp();
                     if (ptx::elect_one()) {

@@ -257,6 +257,13 @@ struct OutBytes {
     static constexpr int value = (OUT == OUT_BF16 || OUT == OUT_F16) ? 2 : 4;
 };
 
+// A TMA store (or add) leaves out the rows beyond the tensor, but along a row it writes whole 16-byte units: where N elements
+// do not end on such a unit it also writes up to 14 bytes of what lies behind them in C's rows (bf16, N = 300 in rows of 352:
+// columns 300 .. 303). So the last, partial box of 128 bytes is not stored by TMA there. Returns the column up to which it is.
+inline int tma_store_columns(long long N, int out_bytes) {
+    return static_cast<int>((N * out_bytes) % 16 == 0 ? N : N - N % (128 / out_bytes));
+}
+
 // Writes 32 consecutive columns of one output row: scale, convert, store (16-byte vectors when the
 // whole chunk is in range and aligned, predicated scalars otherwise).
 template <int KIND, int OUT>
