@@ -166,7 +166,7 @@ int make_operand_map(const void* ptr, uint64_t rows, uint64_t cols, uint64_t ld,
 
 // Output [splits][M][N] (splits == 1 for the final C) with leading dimension ld and slab stride
 // M*ld, elements of 2 or 4 bytes; box = 128 bytes of N x 32 rows x 1 slab, 128-byte swizzle. Stores
-// through it are clipped at N, at M (per slab) and at the slab count.
+// through it end at M (per slab), at the slab count and at the 16-byte unit that N ends in (tma_store_columns).
 int encode_output_map(void* ptr, uint64_t M, uint64_t N, uint64_t ld, uint64_t splits, int out_kind, CUtensorMap* out) {
     CUtensorMapDataType dt;
     uint32_t es;
@@ -712,9 +712,10 @@ int gemm_dispatch_locked(int in_dtype, int out_dtype, int b_layout, const void* 
         ldb_k = plan.ld_relayout;
     }
 
-    // The wide pair kernel stores through TMA only: without a C it can address that way, take the 256 x 256 pairs.
+    // The wide pair kernel stores through TMA only: without a C it can store to the last column that way, take the 256 x 256
+    // pairs.
     if (plan.cfg.wide && (n_extra > 0 || reinterpret_cast<uintptr_t>(C) % 16 != 0 || (ldc * out_bytes) % 16 != 0 ||
-                          g_env.direct_store != 0))
+                          (N * out_bytes) % 16 != 0 || g_env.direct_store != 0))
         plan.cfg.wide = false;
     const Config& cfg = plan.cfg;
     const uint32_t kgroup = static_cast<uint32_t>(plan.kgroup);
@@ -759,7 +760,9 @@ int gemm_dispatch_locked(int in_dtype, int out_dtype, int b_layout, const void* 
         p.split_stride = static_cast<long long>(M) * static_cast<long long>(plan.ldw);
         p.c_vec_ok = 1;
         launch_out = OUT_RAW32;
+        p.n_tma = p.N;  // the slabs' rows are padded to whole units
     } else {
+        p.n_tma = tma_store_columns(p.N, static_cast<int>(out_bytes));
         p.C = C;
         p.ldc = static_cast<long long>(ldc);
         p.split_stride = 0;
@@ -787,6 +790,7 @@ int gemm_dispatch_locked(int in_dtype, int out_dtype, int b_layout, const void* 
         for (int d = 0; d < n_extra; ++d) {
             rc = make_output_map(extra_dsts[d], M, N, static_cast<uint64_t>(ldc), 1, launch_out, &extra.map[d]);
             if (rc != QGEMM_OK) return rc;
+            extra.base[d] = static_cast<uint8_t*>(extra_dsts[d]);
         }
         p.n_extra_dst = n_extra;
     }
@@ -1087,6 +1091,7 @@ int blockscale_dispatch(int out_dtype, int a_layout, int b_layout, const void* A
     std::memset(&tc, 0, sizeof(tc));
     if (reinterpret_cast<uintptr_t>(C) % 16 == 0 && (ldc * out_bytes) % 16 == 0 && g_env.direct_store == 0)
         p.c_tma_ok = make_output_map(C, M, N, ldc, 1, out_kind, &tc) == QGEMM_OK ? 1 : 0;
+    p.n_tma = tma_store_columns(p.N, static_cast<int>(out_bytes));
 
     const long long work = static_cast<long long>(p.m_tiles) * p.n_tiles;
     if (work > 0x7fffffffLL) return QGEMM_ERR_UNSUPPORTED;

@@ -263,7 +263,7 @@ fp8_blockscale_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
                         }
                     }
                 }
-                if (p.c_tma_ok) {
+                if (p.c_tma_ok && n0 < p.n_tma) {
                     if (row0 < p.M) {
                         // one 4 KB staging buffer per warp: the previous store must have read it
                         if (lane == 0) ptx::tma_store_wait_read<0>();
@@ -282,7 +282,7 @@ fp8_blockscale_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
                         }
                     }
                 } else if (row_ok) {
-                    // unaligned C: predicated element stores
+                    // unaligned C, or its last columns beside a unit that TMA would write whole: predicated element stores
                     uint8_t* dst = reinterpret_cast<uint8_t*>(p.C) + (static_cast<long long>(row) * p.ldc + n0) * OB;
 #pragma unroll
                     for (int j = 0; j < CW; ++j) {

@@ -271,6 +271,7 @@ struct BlockScaleParams {
     const float* b_scale;  // [kb_total][n_scale_blocks]
     int* status;
     int c_tma_ok;
+    int n_tma;  // see GemmParams
 };
 cudaError_t launch_fp8_blockscale(int out_kind, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc,
                                   const BlockScaleParams& p, int grid, cudaStream_t stream);

@@ -49,6 +49,7 @@ struct GemmParams {
     int* status;   // device status words: [0] code, [1] cta, [2] role, [3] stage/tile
     int c_vec_ok;  // C base and ldc allow 16-byte vector stores
     int c_tma_ok;  // the C tensor map is valid: the epilogue stores through shared memory + TMA
+    int n_tma;     // with it: boxes of C that begin before this column (tma_store_columns)
     int b_mn_major;  // B is read in place as [K,N] row-major (N contiguous): tmap_b is over [K rows, N cols]
     int n_extra_dst;  // further copies of C written by the same epilogue (CTA-pair kernel only, see ExtraDst)
     // Last-wave split (CTA-pair kernel, splits == 1): work items [0, tail_begin) are whole tiles; item
@@ -96,6 +97,7 @@ struct GemmParams {
 constexpr int kMaxExtraDst = 7;
 struct ExtraDst {
     CUtensorMap map[kMaxExtraDst];
+    uint8_t* base[kMaxExtraDst];
 };
 struct NoExtraDst {
     int unused;
@@ -329,8 +331,8 @@ __device__ __forceinline__ void store_chunk(uint8_t* c_base, long long ldc, long
 constexpr int kEpilogueStagingBytes = 4 * 2 * 4096;
 
 // Drains one accumulator (this warp's 32 rows x BN columns) to C: tcgen05.ld -> scale/convert ->
-// swizzled shared memory -> one TMA store per 128-byte-wide column chunk. The store clips rows and
-// columns that fall outside C. `buf` alternates between the warp's two staging buffers.
+// swizzled shared memory -> one TMA store per 128-byte-wide column chunk that begins before column n_total.
+// The store leaves out rows that fall outside C, and columns but for what tma_store_columns says. `buf` alternates between the warp's two staging buffers.
 template <int KIND, int OUT, int BN>
 __device__ __forceinline__ void epilogue_tma(const CUtensorMap* tmap_c, uint32_t t_addr, int row0, int m_total,
                                              int n_base, int n_total, int split, uint32_t stage_base, int lane,
@@ -392,6 +394,12 @@ __device__ __forceinline__ void epilogue_tma(const CUtensorMap* tmap_c, uint32_t
         }
         buf ^= 1u;
     }
+}
+
+// The first 32-column chunk of a tile that goes to C straight from the registers: none (BN / 32) when TMA stores all of C.
+__device__ __forceinline__ int first_direct_chunk(const GemmParams& p, int n_base, int bn) {
+    if (!p.c_tma_ok) return 0;
+    return p.n_tma < p.N ? max(0, p.n_tma - n_base) / 32 : bn / 32;
 }
 
 // AM = rows of A actually loaded per stage (128, or 64 / 32 when M is that small: the MMA still reads 128 rows,
@@ -696,12 +704,12 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
                             store_chunk<KIND, OUT>(c_base, p.ldc, row, n0, min(32, n_end - n0), p.c_vec_ok != 0, v, alpha);
                     }
                 }
-            } else if (p.c_tma_ok) {
-                epilogue_tma<KIND, OUT, BN>(&tmap_c, t_addr, t.m_blk * kBM + quad * 32, p.M, t.n_blk * BN, p.N, t.split,
-                                            smem_base + L::kOutOffset + (warp - 2) * 8192, lane, alpha, out_buf);
             } else {
+                if (p.c_tma_ok)
+                    epilogue_tma<KIND, OUT, BN>(&tmap_c, t_addr, t.m_blk * kBM + quad * 32, p.M, t.n_blk * BN, p.n_tma, t.split,
+                                                smem_base + L::kOutOffset + (warp - 2) * 8192, lane, alpha, out_buf);
 #pragma unroll 1
-                for (int c = 0; c < BN / 32; ++c) {
+                for (int c = first_direct_chunk(p, t.n_blk * BN, BN); c < BN / 32; ++c) {
                     const int n0 = t.n_blk * BN + c * 32;
                     if (n0 >= p.N) break;  // warp-uniform
                     uint32_t v[32];

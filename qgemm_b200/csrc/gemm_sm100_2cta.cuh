@@ -249,20 +249,24 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
                                                   (item.slot * 2 + static_cast<int>(rank)) * 128 + quad * 32, 0x7fffffff,
                                                   0, BN, t.split, smem_base + L::kOutOffset + (warp - 2) * 8192, lane,
                                                   1.0f, out_buf);
-            } else if (GATHER || p.c_tma_ok) {
-                epilogue_tma<KIND, OUT, BN>(&tmap_c, t_addr, row0, p.M, t.n_blk * BN, p.N, t.split,
-                                            smem_base + L::kOutOffset + (warp - 2) * 8192, lane, alpha, out_buf,
-                                            extra_maps, n_extra);
             } else {
+                if (GATHER || p.c_tma_ok)
+                    epilogue_tma<KIND, OUT, BN>(&tmap_c, t_addr, row0, p.M, t.n_blk * BN, p.n_tma, t.split,
+                                                smem_base + L::kOutOffset + (warp - 2) * 8192, lane, alpha, out_buf,
+                                                extra_maps, n_extra);
 #pragma unroll 1
-                for (int c = 0; c < BN / 32; ++c) {
+                for (int c = first_direct_chunk(p, t.n_blk * BN, BN); c < BN / 32; ++c) {
                     const int n0 = t.n_blk * BN + c * 32;
                     if (n0 >= p.N) break;
                     uint32_t v[32];
                     ptx::tmem_ld_32x32b_x32(t_addr + c * 32, v);
                     ptx::tmem_ld_wait();
-                    if (row < p.M)
+                    if (row < p.M) {
                         store_chunk<KIND, OUT>(c_base, p.ldc, row, n0, min(32, p.N - n0), p.c_vec_ok != 0, v, alpha);
+                        if constexpr (GATHER)
+                            for (int d = 0; d < n_extra; ++d)
+                                store_chunk<KIND, OUT>(extra.base[d], p.ldc, row, n0, min(32, p.N - n0), true, v, alpha);
+                    }
                 }
             }
             ptx::tc_fence_before();

@@ -199,7 +199,7 @@ gemm_tcgen05_wide_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const 
             for (int j = 0; j < 2; ++j) {
                 const int row0 = (t.m_blk * 2 + static_cast<int>(rank)) * 256 + j * 128 + quad * 32;
                 const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + j * BN;
-                epilogue_tma<KIND, OUT, BN>(&tmap_c, t_addr, row0, p.M, t.n_blk * BN, p.N, 0,
+                epilogue_tma<KIND, OUT, BN>(&tmap_c, t_addr, row0, p.M, t.n_blk * BN, p.n_tma, 0,
                                             smem_base + L::kOutOffset + (warp - 2) * 8192, lane, alpha, out_buf);
                 ptx::tc_fence_before();
                 __syncwarp();

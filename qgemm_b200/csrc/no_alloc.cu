@@ -209,6 +209,7 @@ extern "C" int qgemm_mix_gemm_splitk_static(int in_dtype, int out_dtype, const v
     p.status = st->status;
     p.c_vec_ok = 1;
     p.c_tma_ok = 1;
+    p.n_tma = p.N;  // scratch, its rows padded to whole units
     p.test_skip_kb = take_test_skip_kb();
 
     const long long work = static_cast<long long>(p.m_tiles) * p.n_tiles * p.splits;

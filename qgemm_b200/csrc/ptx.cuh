@@ -139,8 +139,8 @@ __device__ __forceinline__ void tma_prefetch_l2_2d(const CUtensorMap* tmap, int 
 }
 
 // 3-D tiled store shared -> global (bulk async-group completion); z selects a slab (split-K partial sums are
-// [split][M][N]). Elements outside the tensor are clipped by the hardware, rows beyond M per slab. Never issued
-// with a negative coordinate.
+// [split][M][N]). The hardware leaves out rows beyond M, per slab, and along a row what lies beyond the last 16-byte unit
+// that the tensor has a part of (tma_store_columns). Never issued with a negative coordinate.
 __device__ __forceinline__ void tma_store_3d(const CUtensorMap* tmap, uint32_t src_smem, int x, int y, int z) {
     asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
                  ::"l"(reinterpret_cast<uint64_t>(tmap)), "r"(src_smem), "r"(x), "r"(y), "r"(z)
@@ -415,7 +415,7 @@ __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.
 __device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_bar) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
-// 3-D tiled fp32 add shared -> global: every element of the box is added once to the tensor's, clipped as a store is.
+// 3-D tiled fp32 add shared -> global: every element of the box is added once to the tensor's, with a store's limits.
 __device__ __forceinline__ void tma_add_3d(const CUtensorMap* tmap, uint32_t src_smem, int x, int y, int z) {
     asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3, %4}], [%1];"
                  ::"l"(reinterpret_cast<uint64_t>(tmap)), "r"(src_smem), "r"(x), "r"(y), "r"(z)
