@@ -119,3 +119,37 @@ def test_a_row_of_nan_stays_in_its_columns(qlib, dev, monkeypatch, out, N):
     finally:
         monkeypatch.undo()
         qlib.lib().qgemm_reload_env()
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 129), (127, 250), (129, 131), (257, 385), (300, 1001), (385, 119)])
+@pytest.mark.parametrize("square", [False, True])
+def test_neighbours_of_aligned_codes_and_values_stay(qlib, dev, rows, cols, square):
+    """Codes and restored values cut out of wider matrices whose rows start on vectors."""
+    x = torch.randn(rows, cols, generator=torch.Generator().manual_seed(rows)).to(dev)
+    want = qlib.quantize_block(x, square=square, form="both")
+
+    def cut(r, c):
+        buf = torch.full((r + 2, -(-c // 16) * 16 + 32), 0x55, dtype=torch.uint8, device=dev)
+        return buf, buf.view(E4M3)[1:r + 1, 16:c + 16]
+
+    def untouched(buf, view):
+        view.view(torch.uint8 if buf.dtype == torch.uint8 else buf.dtype).fill_(0x55)
+        return bool((buf == 0x55).all())
+
+    (qb, q), (tb, qt) = cut(rows, cols), cut(cols, rows)
+    s, st = torch.empty_like(want[1]), torch.empty_like(want[3])
+    for source in (x, x.bfloat16()):
+        ref = qlib.quantize_block(source, square=square, form="both")
+        qlib.quantize_block(source, square=square, form="both", out=(q, s, qt, st))
+        for got, r in zip((q, s, qt, st), ref):
+            assert torch.equal(got.view(torch.uint8), r.view(torch.uint8))
+        assert untouched(qb, q) and untouched(tb, qt)
+    if not square:
+        ref = qlib.requantize_block(want[0], want[1])
+        qlib.requantize_block(want[0], want[1], out=(qt, st))
+        assert torch.equal(qt.view(torch.uint8), ref[0].view(torch.uint8)) and untouched(tb, qt)
+    for out in TYPES:
+        buf = torch.full((rows + 2, -(-cols // 16) * 16 + 32), 0x55, dtype=out, device=dev)
+        back = buf[1:rows + 1, 16:cols + 16]
+        qlib.dequantize_block(want[0], want[1], out=back)
+        assert torch.equal(back, qlib.dequantize_block(want[0], want[1], out)) and untouched(buf, back)

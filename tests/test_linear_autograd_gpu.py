@@ -167,3 +167,52 @@ def test_capture_beside_a_side_streams_graph_that_the_default_stream_used_too(ql
     torch.cuda.synchronize()
     assert torch.equal(got, want)
     del alive
+
+
+@pytest.mark.parametrize("tokens", [1, 2, 129])
+@pytest.mark.parametrize("fin", [1, 15, 128])
+@pytest.mark.parametrize("fout", [1, 17, 129])
+def test_smallest_layers(qlib, dev, tokens, fin, fout):
+    from test_block_e8m0_gpu import _assert_close
+    from test_fp8_linear_gpu import _formula
+
+    from qgemm_b200.linear import fp8_linear
+    x, w = (_data(r, fin, torch.float32, dev, r, 0.5).requires_grad_(True) for r in (tokens, fout))
+    dy = _data(tokens, fout, torch.float32, dev, 3, 0.5)
+    y = fp8_linear(x, w)
+    for got, (ref, mags, k) in zip((y, *torch.autograd.grad(y, (x, w), dy)), _formula(x, w, dy)):
+        _assert_close(got.detach(), ref, mags, k, torch.float32)
+
+
+def test_threads_with_streams_of_their_own(qlib, dev):
+    """Forward and backward in four threads at once."""
+    import threading
+
+    from qgemm_b200.linear import fp8_linear
+    sets = [(_data(100 + i, 512, torch.bfloat16, dev, i, 0.5), _data(300, 512, torch.float32, dev, 9 + i, 0.5)) for i in range(4)]
+
+    def step(x, w):
+        xi, wi = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        y = fp8_linear(xi, wi)
+        return (y.detach(), *torch.autograd.grad(y.sum(), (xi, wi)))
+
+    want = [step(*s) for s in sets]
+    torch.cuda.synchronize()
+    got = [[] for _ in sets]
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                got[i].append(step(*sets[i]))
+        stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i in range(4):
+        assert len(got[i]) == 20
+        for outs in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(outs, want[i]))
