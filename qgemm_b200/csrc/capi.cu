@@ -1180,15 +1180,15 @@ int e8m0_dispatch(int out_dtype, const void* A, size_t lda, const uint8_t* a_sca
     p.accumulate = accumulate != 0;
     p.status = st->status;
 
-    // The tensor cores cut off instead of rounding: with every 32 of K the products and the running sum to multiples of 2^-25
-    // of the largest one's power of two (1 and 32 products of 2^-25 are added exactly, of 2^-26 not at all), and the new sum to
-    // 24 bits. A chain of sums therefore loses up to (33/4 + 1) 2^-23 of its magnitude for every 32 of K, towards zero; for
+    // The tensor cores cut off instead of rounding: with every 32 of K the products and the running sum at multiples of
+    // 2^-25 of the largest one's power of two (1 and 32 products of 2^-25 are added exactly, of 2^-26 not at all), and the
+    // new sum at 24 bits. A chain of sums therefore loses up to (33/4 + 1) 2^-23 of its magnitude for every 32 of K; for
     // values of random sign the norm of the error over that of C was 1.8e-7 over K = 2048 in one chain, 8.6e-7 over 8192,
-    // 2.0e-6 over 16384 and 1.3e-5 over 65536. For a fp32 C, K is taken in parts of at most kE8ChainBlocks blocks a slice, the
-    // later ones added to C with one rounding each. An element's error is then at most 192 * 9.25 * 2^-23 = 2.2e-4 of sum |a b|
-    // however long K is, which takes a first block that outweighs all others (measured: 4.0e-5). 48 blocks, because they
-    // leave values of random sign below 1e-6 with half as much again to spare. (A part has at least half of that, so every
-    // slice of its form has blocks.)
+    // 2.0e-6 over 16384 and 1.3e-5 over 65536. For a fp32 C, K is taken in parts of at most kE8ChainBlocks blocks a slice,
+    // the later ones added to C with one rounding each. An element's error is then at most 192 * 9.25 * 2^-23 = 2.2e-4 of
+    // sum |a b| however long K is, which takes a first block that outweighs all others (measured: 4.0e-5). 48 blocks,
+    // because they leave values of random sign below 1e-6 with half as much again to spare. (A part has at least half of
+    // that, so every slice of its form has blocks.)
     const int kb = (p.K + 127) / 128;
     E8m0Plan plan = plan_e8m0(M, N, K, st->sm_count);
     int parts = 1;

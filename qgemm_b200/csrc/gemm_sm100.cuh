@@ -331,8 +331,9 @@ __device__ __forceinline__ void store_chunk(uint8_t* c_base, long long ldc, long
 constexpr int kEpilogueStagingBytes = 4 * 2 * 4096;
 
 // Drains one accumulator (this warp's 32 rows x BN columns) to C: tcgen05.ld -> scale/convert ->
-// swizzled shared memory -> one TMA store per 128-byte-wide column chunk that begins before column n_total.
-// The store leaves out rows that fall outside C, and columns but for what tma_store_columns says. `buf` alternates between the warp's two staging buffers.
+// swizzled shared memory -> one TMA store per 128-byte-wide column chunk that begins before column n_total. The store leaves
+// out rows that fall outside C, and columns but for what tma_store_columns says. `buf` alternates between the warp's two
+// staging buffers.
 template <int KIND, int OUT, int BN>
 __device__ __forceinline__ void epilogue_tma(const CUtensorMap* tmap_c, uint32_t t_addr, int row0, int m_total,
                                              int n_base, int n_total, int split, uint32_t stage_base, int lane,
